@@ -143,7 +143,8 @@ def prepare(case, seed):
         if own:
             from representax_b200.ops.fp4 import quantize
 
-            d.update({name: quantize(d[name], case["fmt"]) for name in names})
+            # the fused projection keeps its gate and up rows as two parts
+            d.update({name: quantize(d[name], case["fmt"], parts=2 if name == "gate_up" else 1) for name in names})
             if op == "linear" and case["grad"]:
                 d["x"].requires_grad_()
         else:
