@@ -119,6 +119,23 @@ void mx_quantize(const at::Tensor& x, const c10::optional<at::Tensor>& q, const 
 void mx_gemm(const at::Tensor& a, const at::Tensor& sfa, int64_t a_fmt, const at::Tensor& b, const at::Tensor& sfb,
              int64_t b_fmt, int64_t K, at::Tensor& out, int64_t out_mode, const c10::optional<at::Tensor>& bias,
              const c10::optional<at::Tensor>& residual, const at::Tensor& status);
+void gated_forward(const at::Tensor& x, const at::Tensor& gate_up, const c10::optional<at::Tensor>& bias, at::Tensor& h,
+                   const c10::optional<at::Tensor>& saved, const c10::optional<at::Tensor>& exps, int64_t act,
+                   const at::Tensor& status);
+void gated_backward(const at::Tensor& dy, const at::Tensor& down, const at::Tensor& saved, const at::Tensor& exps,
+                    at::Tensor& dz, const at::Tensor& status);
+void few_rows_linear(const at::Tensor& x, const at::Tensor& w, int64_t parts, int64_t act,
+                     const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual, at::Tensor& out,
+                     const at::Tensor& status);
+void fp4_quantize(const at::Tensor& x, int64_t parts, int64_t fmt, at::Tensor& q, at::Tensor& sf,
+                  const c10::optional<at::Tensor>& row_scale);
+void fp4_dequantize(const at::Tensor& q, const at::Tensor& sf, const c10::optional<at::Tensor>& row_scale, int64_t parts,
+                    int64_t fmt, at::Tensor& out);
+void fp4_gemm(const at::Tensor& a, const at::Tensor& a_sf, const c10::optional<at::Tensor>& a_row, const at::Tensor& b,
+              const at::Tensor& b_sf, const c10::optional<at::Tensor>& b_row, int64_t K, int64_t fmt, int64_t parts,
+              int64_t act, const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
+              const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& q_out,
+              const c10::optional<at::Tensor>& q_sf, const at::Tensor& status);
 void sharded_grad_reduce(const at::Tensor& grad_ptrs, int64_t world, int64_t off, int64_t n, at::Tensor& shard,
                          at::Tensor& norm_sq);
 void sharded_adamw(const at::Tensor& shard_grad, int64_t off, int64_t n, const at::Tensor& master_ptrs,
@@ -189,6 +206,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("int4_gemm", &rx::int4_gemm, "tcgen05 GEMM with the packed INT4 weight expanded in the main loop");
   m.def("mx_quantize", &rx::mx_quantize, "MXFP8 quantiser: row-wise and / or transposed 8-bit data + UE8M0 scales");
   m.def("mx_gemm", &rx::mx_gemm, "tcgen05 block-scaled MXFP8 GEMM (kind::mxf8f6f4.block_scale)");
+  m.def("gated_forward", &rx::gated_forward, "tcgen05 gated projection act(x Wg^T) * (x Wu^T), optionally saving for the backward");
+  m.def("gated_backward", &rx::gated_backward, "tcgen05 dz = [dh b | dh a], dh = dy Wd, of the gated feed-forward block");
+  m.def("few_rows_linear", &rx::few_rows_linear, "bf16 (gated) projection of 1 to 64 token rows");
+  m.def("fp4_quantize", &rx::fp4_quantize, "MXFP4 / NVFP4 quantiser");
+  m.def("fp4_dequantize", &rx::fp4_dequantize, "values of MXFP4 / NVFP4 codes and scales");
+  m.def("fp4_gemm", &rx::fp4_gemm, "tcgen05 block-scaled 4-bit GEMM, plain or gated");
   m.def("mnr_tc_argmax", &rx::mnr_tc_argmax, "tcgen05 split-bf16 scores reduced to each row's hardest candidate");
   m.def("sharded_grad_reduce", &rx::sharded_grad_reduce);
   m.def("sharded_adamw", &rx::sharded_adamw);

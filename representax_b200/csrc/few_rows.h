@@ -1,0 +1,48 @@
+// Host interface of the kernels for few token rows (few_rows.cu).
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace rx {
+namespace few {
+
+constexpr int kMaxRows = 64;
+
+enum Kind : int { kBf16 = 0, kMxfp4 = 1, kNvfp4 = 2 };
+
+struct Params {
+  int T, N, K;        // token rows, output columns (per part), contraction
+  int k_blocks;       // pipeline stages along K (64 bf16 or 256 4-bit values each)
+  int gated;          // 1: weight parts [gate; up], output act(g) * u; 0: one part, plain output
+  int act;
+  const __nv_bfloat16* bias;      // [parts * N] or null
+  const __nv_bfloat16* residual;  // [T, N] or null (plain only)
+  int64_t ld_res;
+  __nv_bfloat16* out;             // [T, N], or null with q_out
+  int64_t ld_out;
+  // 4-bit operands
+  const uint8_t* sf_x;
+  const uint8_t* sf_w;
+  int64_t groups;                 // K groups of both scale arrays
+  const float* row_x;             // NVFP4 row factors [T] and [parts * N]
+  const float* row_w;
+  // gated MXFP4 output: codes [T, ld_q] and scales of the next layer's operand
+  uint8_t* q_out;
+  int64_t ld_q;
+  uint8_t* q_sf;
+  int64_t q_groups;
+  int* status;
+  uint64_t timeout_ns;
+};
+
+// Rows of a token tile for T token rows (16, 32 or 64).
+inline int tile_rows(int64_t t) { return t <= 16 ? 16 : (t <= 32 ? 32 : 64); }
+
+// `map_x`: boxes of tile_rows(T) rows x 128 bytes; `map_w`: boxes of 128 rows x 128 bytes.
+cudaError_t launch(int kind, const CUtensorMap& map_x, const CUtensorMap& map_w, const Params& p, int sms, int device,
+                   cudaStream_t stream);
+
+}  // namespace few
+}  // namespace rx

@@ -1,0 +1,561 @@
+// Gated feed-forward block on tcgen05 CTA pairs (bf16 operands, fp32 accumulation).
+//
+//   forward    g = x Wg^T + bg,  u = x Wu^T + bu,  h = act(g) * u
+//   backward   dh = dy Wd,  dz = [dh u act'(g) | dh act(g)]
+//
+// with the framework's fused weight [Wg; Wu] ([2 I, H]) and Wd ([H, I]). The
+// other products of the block (y = h Wd^T, dx = dz [Wg; Wu], the weight
+// gradients) are plain GEMMs of gemm*.cu.
+//
+// Forward: a cluster of two CTAs owns 256 rows x 128 columns of h. The pair's
+// B tile is 256 rows of the fused weight: CTA 0 loads 128 gate rows, CTA 1 the
+// 128 up rows of the same columns, so one M = 256, N = 256 tcgen05.mma leaves g
+// in accumulator columns 0-127 and u in 128-255 of the same TMEM lane, and the
+// thread that holds a row has both operands of the product: z is never
+// written. Without the fusion z costs 4 T I bytes written and read again.
+//
+// For the backward pass the forward saves a = act(g) and b = u act'(g), so the
+// epilogue that produces dz only multiplies: dz = [dh b | dh a]. Both are kept
+// as fp16 with one power of two per row and 32 columns (an exponent byte that
+// puts the block's largest value into [2^14, 2^15)): 11 significant bits down to
+// 2^-29 of that value for the bytes of bf16's 8 bits, so the rounding of dz to bf16 (which the
+// tensor core needs) stays the only one that counts.
+//
+// Backward: the input-gradient GEMM dy Wd with 256 x 256 pair tiles whose
+// epilogue reads the saved tiles (prefetched one 32-column chunk ahead) and
+// stores the two halves of dz; dh is never written.
+//
+// Both are bound by the tensor pipe at training sizes (see the figures at the
+// host entries). The main loops follow the pair kernel of gemm_kernel.cuh: six
+// 32 KB stages, TMA with the 128-byte swizzle, one issuing thread, two
+// accumulator buffers so that an epilogue overlaps the next tile's products.
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "gated_act.cuh"
+#include "gemm_kernel.cuh"
+
+namespace rx {
+namespace gated {
+
+using gemm::BK;
+using gemm::BM;
+using gemm::kEpilogueWarps;
+using gemm::kThreads;
+
+constexpr int kStages = 6;
+constexpr int kTile = BM * BK * 2;  // 16 KB: 128 rows x 64 bf16
+constexpr int kStaging = kEpilogueWarps * 2 * 2048;
+constexpr size_t kSmem = 1024 + kStages * 2 * kTile + kStaging + 256;
+static_assert(kSmem <= 232448, "shared memory beyond the opt-in limit");
+
+struct Params {
+  int M, N, K;  // N: columns of h (forward) or of dh (backward)
+  int m_tiles, n_tiles, num_units;
+  int act;
+  const __nv_bfloat16* bias;  // forward: [2 N] (gate, up) or null
+  const __half* saved_b;      // backward: b [M, N], a [M, N] with row stride ld_saved
+  const __half* saved_a;
+  int64_t ld_saved;
+  uint16_t* exps;             // [M, ceil(N / 32)]: low byte the block exponent of b, high byte that of a
+  int64_t ld_exps;
+  int* status;
+  uint64_t timeout_ns;
+};
+
+// Exponent byte e of a block with largest magnitude `top`: values are stored
+// times 2^(141 - e) and read back times 2^(e - 141). Clamped so that both
+// factors are normal floats; an infinite or NaN value keeps being one.
+__device__ __forceinline__ uint32_t block_byte(float top) {
+  return min(max((__float_as_uint(top) >> 23) & 0xffu, 15u), 254u);
+}
+__device__ __forceinline__ float store_factor(uint32_t e) { return __uint_as_float((268u - e) << 23); }
+__device__ __forceinline__ float load_factor(uint32_t e) { return __uint_as_float((e - 14u) << 23); }
+
+// Row `lane` of a 32 x 32 tile of 16-bit values staged for a tile store (64-byte swizzle).
+__device__ __forceinline__ void stage_half32(uint8_t* buf, int lane, const float (&v)[32], float f) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint4 w;
+    __half2* h = reinterpret_cast<__half2*>(&w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(v[q * 8 + 2 * j] * f, v[q * 8 + 2 * j + 1] * f);
+    *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16)) = w;
+  }
+}
+__device__ __forceinline__ void read_half32(const uint8_t* buf, int lane, float (&v)[32], float f) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint4 w = *reinterpret_cast<const uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16));
+    const __half2* h = reinterpret_cast<const __half2*>(&w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = __half22float2(h[j]);
+      v[q * 8 + 2 * j] = t.x * f;
+      v[q * 8 + 2 * j + 1] = t.y * f;
+    }
+  }
+}
+
+// One warp's staged stores: two 2 KB buffers used in turn; a buffer is free
+// once at most one of the lane's committed stores is still reading.
+struct Staging {
+  uint8_t* base;
+  uint32_t seq = 0;
+  __device__ __forceinline__ uint8_t* next(int lane) {
+    if (lane == 0) tma_store_wait_read<1>();
+    __syncwarp();
+    return base + (seq++ & 1) * 2048;
+  }
+  __device__ __forceinline__ void store(const CUtensorMap* map, const uint8_t* buf, int x, int y, int lane) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(map, buf, x, y);
+      tma_store_commit();
+    }
+  }
+};
+
+__device__ __forceinline__ void add_bias32(const __nv_bfloat16* bias, int n_base, int n, float (&v)[32]) {
+  if (n_base + 32 <= n) {
+    float b[32];
+    gemm::load_bf16x32(bias + n_base, b);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] += b[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] += n_base + i < n ? __bfloat162float(bias[n_base + i]) : 0.f;
+  }
+}
+
+// MODE 0: forward; 1: forward that saves a and b; 2: backward (dz).
+template <int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+    gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                 const __grid_constant__ CUtensorMap tmOut0, const __grid_constant__ CUtensorMap tmOut1,
+                 const __grid_constant__ CUtensorMap tmOut2, const Params p) {
+  constexpr bool kBackward = MODE == 2;
+  constexpr bool kSave = MODE == 1;
+  constexpr int kTileCols = kBackward ? 256 : 128;  // output columns of a tile
+  constexpr uint32_t kTmemCols = 512;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = base;
+  uint8_t* sB = base + kStages * kTile;
+  uint8_t* sC = sB + kStages * kTile;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sC + kStaging);
+  uint64_t* empty = full + kStages;
+  uint64_t* tfull = empty + kStages;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = warp_id(), lane = lane_id();
+  const int rank = static_cast<int>(cluster_ctarank());
+  const bool leader = rank == 0;
+  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 2 * kEpilogueWarps);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_map(&tmA);
+    tma_prefetch_map(&tmB);
+    tma_prefetch_map(&tmOut0);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, kTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync_all();  // both CTAs' barriers are initialised before any remote use
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int k_blocks = (p.K + BK - 1) / BK;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      const uint32_t full_leader0 = mapa_shared(smem_u32(&full[0]), 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int u = cluster; ok && u < p.num_units; u += clusters) {
+        const int m = (u / p.n_tiles) * (2 * BM) + rank * BM;
+        const int n0 = (u % p.n_tiles) * kTileCols;
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (*abort_flag || !mbar_wait(&empty[stage], phase ^ 1, p.timeout_ns)) {
+            report_status(p.status, kStatusTimeoutProducer);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          if (leader) mbar_arrive_expect_tx(&full[stage], 4 * kTile);  // both CTAs' A and B halves
+          const uint32_t bar = full_leader0 + stage * 8;
+          uint8_t* a_dst = sA + stage * kTile;
+          uint8_t* b_dst = sB + stage * kTile;
+          tma_load_2d_pair(a_dst, &tmA, bar, kb * BK, m);
+          if constexpr (kBackward) {  // Wd [K, N] is MN-major: two 64 x 64 boxes
+            tma_load_2d_pair(b_dst, &tmB, bar, n0 + rank * 128, kb * BK);
+            tma_load_2d_pair(b_dst + 8192, &tmB, bar, n0 + rank * 128 + 64, kb * BK);
+          } else {  // CTA 0: gate rows, CTA 1: up rows of the same columns
+            tma_load_2d_pair(b_dst, &tmB, bar, kb * BK, n0 + rank * p.N);
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // every load was consumed once the MMAs of its stage have committed
+      for (int s = 0; s < kStages; ++s) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, p.timeout_ns)) {
+          report_status(p.status, kStatusTimeoutDrain);
+          break;
+        }
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (even CTA)
+    if (leader && lane == 0) {
+      constexpr uint32_t IDESC = idesc_bf16_f32(2 * BM, 256, false, kBackward);
+      int stage = 0, local = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int u = cluster; ok && u < p.num_units; u += clusters, ++local) {
+        const int acc = local & 1;
+        if (*abort_flag || !mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, p.timeout_ns)) {
+          report_status(p.status, kStatusTimeoutMma);
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * 256);
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (*abort_flag || !mbar_wait(&full[stage], phase, p.timeout_ns)) {
+            report_status(p.status, kStatusTimeoutMma);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a = smem_u32(sA + stage * kTile), b = smem_u32(sB + stage * kTile);
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk)
+            umma_f16_ss_pair(d_tmem, smem_desc_sw128(a + kk * 32, 16, 1024),
+                             kBackward ? smem_desc_sw128(b + kk * 2048, 8192, 1024)
+                                       : smem_desc_sw128(b + kk * 32, 16, 1024),
+                             IDESC, (kb > 0 || kk > 0) ? 1u : 0u);
+          umma_commit_pair(&empty[stage], 0x3);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        umma_commit_pair(&tfull[acc], 0x3);
+      }
+      umma_commit_pair(drain, 0x3);
+    }
+    if (lane == 0 && !mbar_wait(drain, 0, p.timeout_ns)) report_status(p.status, kStatusTimeoutDrain);
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue (both CTAs)
+    const int quad = warp & 3;
+    constexpr int kChunks = kTileCols / 32 / (kEpilogueWarps / 4);
+    const int chunk0 = ((warp - 2) / 4) * kChunks;
+    const uint32_t tempty_leader = mapa_shared(smem_u32(&tempty[0]), 0);
+    Staging staging{sC + (warp - 2) * 4096};
+    int local = 0;
+    for (int u = cluster; u < p.num_units; u += clusters, ++local) {
+      const int acc = local & 1;
+      const int row0 = (u / p.n_tiles) * (2 * BM) + rank * BM + quad * 32;  // this warp's 32 rows
+      const int n0 = (u % p.n_tiles) * kTileCols;
+      const int m = row0 + lane;
+      uint4 next_b[4], next_a[4];
+      uint32_t next_e = 0;
+      if constexpr (kBackward) {  // the first chunk's saved tiles, in flight while the products finish
+        const int n = n0 + chunk0 * 32;
+        if (n < p.N && row0 < p.M) {
+          gemm::warp_fetch_tile32(reinterpret_cast<const __nv_bfloat16*>(p.saved_b), p.ld_saved, row0, n, p.M, p.N, lane,
+                                  next_b);
+          gemm::warp_fetch_tile32(reinterpret_cast<const __nv_bfloat16*>(p.saved_a), p.ld_saved, row0, n, p.M, p.N, lane,
+                                  next_a);
+          if (m < p.M) next_e = p.exps[static_cast<int64_t>(m) * p.ld_exps + (n >> 5)];
+        }
+      }
+      bool ok = (*abort_flag == 0) && mbar_wait(&tfull[acc], (local >> 1) & 1, p.timeout_ns);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        if (lane == 0) report_status(p.status, kStatusTimeoutEpilogue);
+        *abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * 256);
+#pragma unroll 1
+      for (int c = chunk0; c < chunk0 + kChunks; ++c) {
+        const int n = n0 + c * 32;
+        const bool live = n < p.N && row0 < p.M;  // warp-uniform
+        if constexpr (kBackward) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(t_row + c * 32, r);
+          uint4 cur_b[4], cur_a[4];
+          const uint32_t e = next_e;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            cur_b[q] = next_b[q];
+            cur_a[q] = next_a[q];
+          }
+          if (c + 1 < chunk0 + kChunks && n + 32 < p.N && row0 < p.M) {
+            gemm::warp_fetch_tile32(reinterpret_cast<const __nv_bfloat16*>(p.saved_b), p.ld_saved, row0, n + 32, p.M, p.N,
+                                    lane, next_b);
+            gemm::warp_fetch_tile32(reinterpret_cast<const __nv_bfloat16*>(p.saved_a), p.ld_saved, row0, n + 32, p.M, p.N,
+                                    lane, next_a);
+            if (m < p.M) next_e = p.exps[static_cast<int64_t>(m) * p.ld_exps + ((n + 32) >> 5)];
+          }
+          tmem_ld_wait();
+          if (!live) continue;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint8_t* buf = staging.next(lane);
+            float v[32];
+            gemm::warp_put_tile32_sw64(buf, lane, half == 0 ? cur_b : cur_a);
+            __syncwarp();
+            // rows past the end hold zeros and an exponent byte that reads as the smallest factor
+            read_half32(buf, lane, v, load_factor(max(half == 0 ? e & 0xffu : e >> 8, 15u)));
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= __uint_as_float(r[i]);
+            gemm::stage_row32_sw64(buf, lane, v);
+            staging.store(half == 0 ? &tmOut0 : &tmOut1, buf, n, row0, lane);
+          }
+        } else {
+          uint32_t rg[32], ru[32];
+          tmem_ld_32x32b_x32(t_row + c * 32, rg);
+          tmem_ld_32x32b_x32(t_row + 128 + c * 32, ru);
+          tmem_ld_wait();
+          if (!live) continue;
+          float g[32], v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            g[i] = __uint_as_float(rg[i]);
+            v[i] = __uint_as_float(ru[i]);
+          }
+          if (p.bias != nullptr) {
+            add_bias32(p.bias, n, p.N, g);
+            add_bias32(p.bias + p.N, n, p.N, v);
+          }
+          if (n + 32 > p.N) {  // columns past the end (the gate side holds up rows there) count as zero
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (n + i >= p.N) g[i] = v[i] = 0.f;
+          }
+          if constexpr (kSave) {
+            float b[32];
+            float top_a = 0.f, top_b = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              float value, grad;
+              act_value_grad(g[i], p.act, value, grad);
+              g[i] = value;
+              b[i] = v[i] * grad;
+              v[i] *= value;
+              top_a = fmaxf(top_a, fabsf(g[i]));
+              top_b = fmaxf(top_b, fabsf(b[i]));
+            }
+            const uint32_t ea = block_byte(top_a), eb = block_byte(top_b);
+            if (m < p.M) p.exps[static_cast<int64_t>(m) * p.ld_exps + (n >> 5)] = static_cast<uint16_t>(eb | (ea << 8));
+            uint8_t* buf = staging.next(lane);
+            gemm::stage_row32_sw64(buf, lane, v);
+            staging.store(&tmOut0, buf, n, row0, lane);
+            buf = staging.next(lane);
+            stage_half32(buf, lane, b, store_factor(eb));
+            staging.store(&tmOut1, buf, n, row0, lane);
+            buf = staging.next(lane);
+            stage_half32(buf, lane, g, store_factor(ea));
+            staging.store(&tmOut2, buf, n, row0, lane);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= act_value(g[i], p.act);
+            uint8_t* buf = staging.next(lane);
+            gemm::stage_row32_sw64(buf, lane, v);
+            staging.store(&tmOut0, buf, n, row0, lane);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(tempty_leader + acc * 8);
+    }
+    if (lane == 0) tma_store_wait<0>();  // every tile store has landed before the CTA exits
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // no CTA leaves while its peer may still signal it
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc_pair(tmem_base, kTmemCols);
+}
+
+template <int MODE>
+void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& o0, const CUtensorMap& o1,
+            const CUtensorMap& o2, const Params& p, int device, cudaStream_t stream) {
+  auto kern = gated_kernel<MODE>;
+  static bool configured[64] = {false};
+  if (device < 0 || device >= 64 || !configured[device]) {
+    RX_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem)));
+    if (device >= 0 && device < 64) configured[device] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * std::min(p.num_units, num_sms(device) / 2));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  RX_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, o0, o1, o2, p));
+}
+
+static void check_rows(const at::Tensor& t, const char* name, int64_t rows, int64_t cols, int device) {
+  RX_CHECK(t.is_cuda() && t.get_device() == device, name, " must be on the device of the first operand");
+  RX_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols && t.stride(1) == 1, name, " must be a row-major [",
+           rows, ", ", cols, "]");
+  RX_CHECK((t.stride(0) * t.element_size()) % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name,
+           " rows must be 16-byte aligned");
+}
+
+static void check_sizes(int64_t T, int64_t H, int64_t I) {
+  RX_CHECK(T > 0 && H > 0 && I > 0, "empty gated feed-forward");
+  RX_CHECK(H % 8 == 0 && I % 8 == 0, "hidden and intermediate sizes must be multiples of 8");
+  RX_CHECK(T < (1ll << 31) - 256 && H < (1ll << 30) && I < (1ll << 30), "gated feed-forward too large");
+}
+
+}  // namespace gated
+
+// h [T, I] = act(x Wg^T + bg) * (x Wu^T + bu) for x [T, H] and gate_up = [Wg; Wu] [2 I, H].
+// With `saved` (fp16 [T, 2 I]: b, then a) and `exps` (int16 [T, ceil(I / 32)]) it also keeps what
+// gated_backward reads.
+void gated_forward(const at::Tensor& x, const at::Tensor& gate_up, const c10::optional<at::Tensor>& bias,
+                   at::Tensor& h, const c10::optional<at::Tensor>& saved, const c10::optional<at::Tensor>& exps,
+                   int64_t act, const at::Tensor& status) {
+  check_bf16(x, "x");
+  check_bf16(gate_up, "gate_up");
+  check_bf16(h, "h");
+  RX_CHECK(x.dim() == 2 && gate_up.dim() == 2, "x and gate_up must be matrices");
+  const int64_t T = x.size(0), H = x.size(1), I = gate_up.size(0) / 2;
+  const int dev = x.get_device();
+  RX_CHECK(gate_up.size(0) == 2 * I, "gate_up must have an even number of rows");
+  gated::check_sizes(T, H, I);
+  gated::check_rows(x, "x", T, H, dev);
+  gated::check_rows(gate_up, "gate_up", 2 * I, H, dev);
+  gated::check_rows(h, "h", T, I, dev);
+  RX_CHECK(act >= 0 && act <= 3, "unknown activation code ", act);
+  RX_CHECK(saved.has_value() == exps.has_value(), "give saved and exps together");
+  gated::Params p{};
+  p.M = static_cast<int>(T);
+  p.N = static_cast<int>(I);
+  p.K = static_cast<int>(H);
+  p.m_tiles = static_cast<int>((T + 255) / 256);
+  p.n_tiles = static_cast<int>((I + 127) / 128);
+  RX_CHECK(static_cast<int64_t>(p.m_tiles) * p.n_tiles < (1ll << 31), "too many tiles");
+  p.num_units = p.m_tiles * p.n_tiles;
+  p.act = static_cast<int>(act);
+  p.status = status_ptr(status);
+  p.timeout_ns = kWaitBudgetNs;
+  if (bias.has_value()) {
+    check_bf16(*bias, "bias");
+    RX_CHECK(bias->get_device() == dev && bias->dim() == 1 && bias->numel() == 2 * I && bias->is_contiguous() &&
+                 reinterpret_cast<uintptr_t>(bias->data_ptr()) % 16 == 0,
+             "bias must be a contiguous 16-byte aligned [2 I] vector");
+    p.bias = reinterpret_cast<const __nv_bfloat16*>(bias->data_ptr());
+  }
+  c10::cuda::CUDAGuard guard(dev);
+  const CUtensorMap ta = make_tmap_2d_bf16(x.data_ptr(), T, H, x.stride(0), 64, gemm::BM);
+  const CUtensorMap tb = make_tmap_2d_bf16(gate_up.data_ptr(), 2 * I, H, gate_up.stride(0), 64, 128);
+  const CUtensorMap th = make_tmap_2d_bf16_store(h.data_ptr(), T, I, h.stride(0));
+  auto stream = at::cuda::getCurrentCUDAStream(dev).stream();
+  if (!saved.has_value()) {
+    gated::launch<0>(ta, tb, th, th, th, p, dev, stream);
+    return;
+  }
+  RX_CHECK(saved->scalar_type() == at::kHalf, "saved must be float16");
+  gated::check_rows(*saved, "saved", T, 2 * I, dev);
+  RX_CHECK(exps->is_cuda() && exps->get_device() == dev && exps->scalar_type() == at::kShort && exps->is_contiguous() &&
+               exps->dim() == 2 && exps->size(0) == T && exps->size(1) == (I + 31) / 32,
+           "exps must be a contiguous int16 [T, ceil(I / 32)]");
+  p.exps = reinterpret_cast<uint16_t*>(exps->data_ptr());
+  p.ld_exps = exps->size(1);
+  auto* sp = reinterpret_cast<__half*>(saved->data_ptr());
+  const CUtensorMap tb_out = make_tmap_2d_bf16_store(sp, T, I, saved->stride(0));
+  const CUtensorMap ta_out = make_tmap_2d_bf16_store(sp + I, T, I, saved->stride(0));
+  gated::launch<1>(ta, tb, th, tb_out, ta_out, p, dev, stream);
+}
+
+// dz [T, 2 I] = [dh b | dh a] with dh = dy Wd (dy [T, H], down [H, I]) and what gated_forward saved.
+void gated_backward(const at::Tensor& dy, const at::Tensor& down, const at::Tensor& saved, const at::Tensor& exps,
+                    at::Tensor& dz, const at::Tensor& status) {
+  check_bf16(dy, "dy");
+  check_bf16(down, "down");
+  check_bf16(dz, "dz");
+  RX_CHECK(dy.dim() == 2 && down.dim() == 2, "dy and down must be matrices");
+  const int64_t T = dy.size(0), H = dy.size(1), I = down.size(1);
+  const int dev = dy.get_device();
+  gated::check_sizes(T, H, I);
+  gated::check_rows(dy, "dy", T, H, dev);
+  gated::check_rows(down, "down", H, I, dev);
+  gated::check_rows(dz, "dz", T, 2 * I, dev);
+  RX_CHECK(saved.scalar_type() == at::kHalf, "saved must be float16");
+  gated::check_rows(saved, "saved", T, 2 * I, dev);
+  RX_CHECK(exps.is_cuda() && exps.get_device() == dev && exps.scalar_type() == at::kShort && exps.is_contiguous() &&
+               exps.dim() == 2 && exps.size(0) == T && exps.size(1) == (I + 31) / 32,
+           "exps must be a contiguous int16 [T, ceil(I / 32)]");
+  gated::Params p{};
+  p.M = static_cast<int>(T);
+  p.N = static_cast<int>(I);
+  p.K = static_cast<int>(H);
+  p.m_tiles = static_cast<int>((T + 255) / 256);
+  p.n_tiles = static_cast<int>((I + 255) / 256);
+  RX_CHECK(static_cast<int64_t>(p.m_tiles) * p.n_tiles < (1ll << 31), "too many tiles");
+  p.num_units = p.m_tiles * p.n_tiles;
+  p.status = status_ptr(status);
+  p.timeout_ns = kWaitBudgetNs;
+  p.saved_b = reinterpret_cast<const __half*>(saved.data_ptr());
+  p.saved_a = p.saved_b + I;
+  p.ld_saved = saved.stride(0);
+  p.exps = reinterpret_cast<uint16_t*>(exps.data_ptr());
+  p.ld_exps = exps.size(1);
+  c10::cuda::CUDAGuard guard(dev);
+  const CUtensorMap ta = make_tmap_2d_bf16(dy.data_ptr(), T, H, dy.stride(0), 64, gemm::BM);
+  const CUtensorMap tb = make_tmap_2d_bf16(down.data_ptr(), H, I, down.stride(0), 64, 64);
+  auto* zp = reinterpret_cast<__nv_bfloat16*>(dz.data_ptr());
+  const CUtensorMap t0 = make_tmap_2d_bf16_store(zp, T, I, dz.stride(0));
+  const CUtensorMap t1 = make_tmap_2d_bf16_store(zp + I, T, I, dz.stride(0));
+  gated::launch<2>(ta, tb, t0, t1, t1, p, dev, at::cuda::getCurrentCUDAStream(dev).stream());
+}
+
+}  // namespace rx

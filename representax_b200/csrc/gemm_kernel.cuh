@@ -27,6 +27,7 @@
 // backward; this kernel replaces both.
 #pragma once
 #include "common.h"
+#include "gelu.cuh"
 #include "philox.cuh"
 #include "sm100.cuh"
 
@@ -86,35 +87,6 @@ struct Params {
 // (kind::f8f6f4), KIND - 1 = (a_fmt | b_fmt << 1) with 0 = E4M3, 1 = E5M2.
 constexpr int kKindBf16 = 0;
 constexpr int fp8_kind(int a_fmt, int b_fmt) { return 1 + (a_fmt | (b_fmt << 1)); }
-
-// GELU (erf form) and its derivative from one exponential: the normal CDF
-// Phi(x) = (1 + erf(x / sqrt 2)) / 2 uses the rational approximation of
-// Abramowitz & Stegun, Handbook of Mathematical Functions, eq. 7.1.26
-// (|error of erf| <= 1.5e-7, far below bf16's resolution), whose exp(-u^2)
-// factor at u = |x| / sqrt 2 is exp(-x^2 / 2), the same exponential the normal
-// density phi(x) needs. gelu = x Phi(x); gelu' = Phi(x) + x phi(x).
-__device__ __forceinline__ void gelu_and_grad(float x, float& gelu, float& grad) {
-  const float u = fabsf(x) * 0.70710678118654752440f;
-  float t;  // 1 / (1 + p u) by the approximate reciprocal (a few ulp, far below bf16's resolution)
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f, u, 1.0f)));
-  float poly = fmaf(1.061405429f, t, -1.453152027f);
-  poly = fmaf(poly, t, 1.421413741f);
-  poly = fmaf(poly, t, -0.284496736f);
-  poly = fmaf(poly, t, 0.254829592f);
-  poly *= t;
-  float e;  // exp(-x^2 / 2) = 2^(-x^2 / 2 * log2(e))
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-0.72134752044448170368f * x * x));
-  const float erf_u = 1.0f - poly * e;  // erf(|x| / sqrt 2)
-  const float cdf = 0.5f + 0.5f * copysignf(erf_u, x);
-  gelu = x * cdf;
-  grad = fmaf(x * 0.39894228040143267794f, e, cdf);
-}
-
-__device__ __forceinline__ float gelu_erf(float x) {
-  float g, d;
-  gelu_and_grad(x, g, d);
-  return g;
-}
 
 __device__ __forceinline__ void load_bf16x32(const __nv_bfloat16* src, float (&v)[32]) {
   const uint4* s = reinterpret_cast<const uint4*>(src);

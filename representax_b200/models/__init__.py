@@ -13,6 +13,7 @@ from .adapters import (
 )
 from .bert import BertBatch, BertCheckpointAdapter, BertConfig, BertEncoder, build_bert
 from .clip import CLIPBatch, CLIPCheckpointAdapter, CLIPConfig, CLIPEncoder, build_clip
+from .fp4 import FP4Weight, quantize_linears_fp4
 from .jina_v5 import JinaV5CheckpointAdapter, JinaV5TextEncoder, load_jina_v5_small_text_encoder
 from .modernvbert import (
     ModernVBERTBatch,
@@ -55,10 +56,10 @@ __all__ = [
     "Qwen3VLConfig", "Qwen3VLEncoder", "Qwen3VLReranker", "build_clip", "build_modernvbert",
     "load_jina_v5_small_text_encoder",
     "BertBatch", "BertCheckpointAdapter", "BertConfig", "BertEncoder", "DenoisingAutoEncoder", "DenseEncoder",
-    "EncoderPair", "MPNetCheckpointAdapter", "MPNetConfig", "MPNetEncoder", "POOLING_MODES", "PackedTokens",
+    "EncoderPair", "FP4Weight", "MPNetCheckpointAdapter", "MPNetConfig", "MPNetEncoder", "POOLING_MODES", "PackedTokens",
     "PairClassifier", "Processor", "QuantizedLoRAWeight", "SentenceBatch", "SentenceDense", "SentenceEncoder",
     "SentenceNormalize", "SentencePooling", "TokenBatch", "TokenReconstructionDecoder", "apply_quantized_lora",
     "build_bert", "build_mpnet", "lora_parameter_filter", "make_audio_processor", "make_image_processor",
     "make_media_processor", "make_text_processor", "make_video_processor", "merge_quantized_lora", "pack_int4_rows",
-    "pack_tokens", "select_static_shape_bucket", "unpack_int4_rows",
+    "pack_tokens", "quantize_linears_fp4", "select_static_shape_bucket", "unpack_int4_rows",
 ]

@@ -63,8 +63,7 @@ class ModernBertLayer(nn.Module):
         a = N.qkv_attention(qkv, seg, heads=cfg.num_attention_heads, pos=pos, inv_freq=inv_freq, window=window)
         h = N.linear(a, self.Wo, residual=h)
         x = N.layer_norm(h, self.mlp_norm, None, cfg.norm_epsilon)
-        g = N.gated_activation(N.linear(x, self.Wi), cfg.hidden_activation)
-        return N.linear(g, self.mlp_Wo, residual=h)
+        return N.gated_mlp(x, self.Wi, self.mlp_Wo, cfg.hidden_activation, residual=h)
 
 
 class ModernBertTextTower(nn.Module):

@@ -229,8 +229,7 @@ class _OmniVisionBlock(nn.Module):
                             axis_of=axis)
         h = N.linear(a, self.proj_w, self.proj_b, residual=h)
         x = N.rms_norm(h, self.n2, 1e-6)
-        m = N.gated_activation(N.linear(x, self.gate_up_w, self.gate_up_b), cfg.hidden_activation)
-        return N.linear(m, self.down_w, self.down_b, residual=h)
+        return N.gated_mlp(x, self.gate_up_w, self.down_w, cfg.hidden_activation, self.gate_up_b, self.down_b, residual=h)
 
 
 class OmniVisionTower(nn.Module):

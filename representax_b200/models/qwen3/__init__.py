@@ -114,8 +114,7 @@ class Qwen3DecoderLayer(nn.Module):
                             q_norm=self.q_norm, k_norm=self.k_norm, norm_eps=cfg.norm_epsilon, causal=True)
         h = N.linear(a, self.o_proj, residual=h)
         x = N.rms_norm(h, self.post_norm, cfg.norm_epsilon)
-        g = N.gated_activation(N.linear(x, self.gate_up), "silu")
-        return N.linear(g, self.down, residual=h)
+        return N.gated_mlp(x, self.gate_up, self.down, "silu", residual=h)
 
 
 class Qwen3TextTower(nn.Module):

@@ -17,6 +17,9 @@ src/representax/models/modernvbert/model.py:82-112.
 from __future__ import annotations
 
 import math
+from collections.abc import Iterator
+from contextlib import contextmanager
+from contextvars import ContextVar
 from dataclasses import dataclass
 
 import torch
@@ -109,7 +112,12 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     scaling."""
 
     from representax_b200.models.adapters import QuantizedLoRAWeight
+    from representax_b200.models.fp4 import FP4Weight
 
+    if isinstance(weight, FP4Weight):
+        from .fp4 import linear_fp4
+
+        return linear_fp4(x, weight.operand, bias, residual)
     if isinstance(weight, QuantizedLoRAWeight):
         if native(x) and x.shape[1] % 16 == 0 and weight.output_size % 8 == 0:
             return weight.linear_native(x.contiguous(), bias, residual)
@@ -481,6 +489,47 @@ def gated_activation(z: torch.Tensor, name: str) -> torch.Tensor:
     return (_act_reference(zf[:, :width], name) * zf[:, width:]).to(z.dtype)
 
 
+# ----------------------------------------------------------- feed-forward
+_FUSED_FEED_FORWARD: ContextVar[bool] = ContextVar("representax_b200_fused_feed_forward", default=False)
+
+
+@contextmanager
+def fused_feed_forward(enabled: bool = True) -> Iterator[None]:
+    """Run the gated feed-forward blocks of models called inside as the fused kernels of ``ops.ffn``.
+
+    Off by default: the separate layers round the projections to bf16 where the
+    fused block keeps them in fp32, so results differ in the last bits."""
+
+    token = _FUSED_FEED_FORWARD.set(enabled)
+    try:
+        yield
+    finally:
+        _FUSED_FEED_FORWARD.reset(token)
+
+
+def gated_mlp(x: torch.Tensor, gate_up, down, name: str, gate_up_bias: torch.Tensor | None = None,
+              down_bias: torch.Tensor | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """A layer's gated feed-forward block, ``(act(g) * u) down^T`` with ``[g u] = x gate_up^T``.
+
+    4-bit weights run the 4-bit block of ``ops.fp4``; plain weights the separate
+    layers, or the fused kernels inside :func:`fused_feed_forward` (not under an fp8 policy)."""
+
+    from representax_b200.models.fp4 import FP4Weight
+
+    if isinstance(gate_up, FP4Weight) and isinstance(down, FP4Weight):
+        from .fp4 import gated_feed_forward_fp4
+
+        return gated_feed_forward_fp4(x, gate_up.operand, down.operand, activation=name, gate_up_bias=gate_up_bias,
+                                      down_bias=down_bias, residual=residual)
+    if (_FUSED_FEED_FORWARD.get() and isinstance(gate_up, torch.Tensor) and isinstance(down, torch.Tensor)
+            and native(x) and not _fp8_matrices()):
+        from .ffn import gated_feed_forward
+
+        return gated_feed_forward(x, gate_up, down, activation=name, gate_up_bias=gate_up_bias, down_bias=down_bias,
+                                  residual=residual)
+    return linear(gated_activation(linear(x, gate_up, gate_up_bias), name), down, down_bias, residual=residual)
+
+
 # ---------------------------------------------------------------- pooling
 def pool_rows(h: torch.Tensor, seg: Segments, mode: str = "mean", normalize: bool = True) -> torch.Tensor:
     """Per-sequence mean / first / last row of packed hidden states (fp32)."""
@@ -521,6 +570,7 @@ def sinusoid_table(n: int, dim: int) -> torch.Tensor:
     return torch.cat([torch.sin(ang), torch.cos(ang)], 1).float()
 
 
-__all__ = ["ACT_CODES", "Segments", "activation", "attention", "gated_activation", "layer_norm", "linear",
+__all__ = ["ACT_CODES", "Segments", "activation", "attention", "fused_feed_forward", "gated_activation", "gated_mlp",
+           "layer_norm", "linear",
            "mrope_axis_table", "native", "pool_rows", "qkv_attention", "rms_norm", "rope", "rope_inv_freq", "scatter_rows",
            "sinusoid_table", "weight_as"]
