@@ -126,16 +126,37 @@ void gated_backward(const at::Tensor& dy, const at::Tensor& down, const at::Tens
                     at::Tensor& dz, const at::Tensor& status);
 void few_rows_linear(const at::Tensor& x, const at::Tensor& w, int64_t parts, int64_t act,
                      const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual, at::Tensor& out,
-                     const at::Tensor& status);
-void fp4_quantize(const at::Tensor& x, int64_t parts, int64_t fmt, at::Tensor& q, at::Tensor& sf,
-                  const c10::optional<at::Tensor>& row_scale);
+                     bool after_producer, const at::Tensor& status);
+std::vector<at::Tensor> gated_ffn_forward(const at::Tensor& x, const at::Tensor& gate_up, const at::Tensor& down,
+                                          const c10::optional<at::Tensor>& gate_up_bias,
+                                          const c10::optional<at::Tensor>& down_bias,
+                                          const c10::optional<at::Tensor>& residual, int64_t act, bool save,
+                                          const at::Tensor& status);
+std::vector<at::Tensor> gated_ffn_backward(const at::Tensor& dy, const c10::optional<at::Tensor>& x,
+                                           const c10::optional<at::Tensor>& h, const at::Tensor& gate_up,
+                                           const at::Tensor& down, const c10::optional<at::Tensor>& saved,
+                                           const c10::optional<at::Tensor>& exps, const std::vector<bool>& need,
+                                           const std::vector<c10::optional<at::Tensor>>& acc,
+                                           const std::vector<at::ScalarType>& like, const at::Tensor& status);
+std::vector<at::Tensor> fp4_quantize(const at::Tensor& x, int64_t parts, int64_t fmt);
 void fp4_dequantize(const at::Tensor& q, const at::Tensor& sf, const c10::optional<at::Tensor>& row_scale, int64_t parts,
                     int64_t fmt, at::Tensor& out);
-void fp4_gemm(const at::Tensor& a, const at::Tensor& a_sf, const c10::optional<at::Tensor>& a_row, const at::Tensor& b,
-              const at::Tensor& b_sf, const c10::optional<at::Tensor>& b_row, int64_t K, int64_t fmt, int64_t parts,
-              int64_t act, const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
-              const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& q_out,
-              const c10::optional<at::Tensor>& q_sf, const at::Tensor& status);
+at::Tensor fp4_gemm(const at::Tensor& a, const at::Tensor& a_sf, const c10::optional<at::Tensor>& a_row, const at::Tensor& b,
+                    const at::Tensor& b_sf, const c10::optional<at::Tensor>& b_row, int64_t parts, int64_t K, int64_t fmt,
+                    const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
+                    const at::Tensor& status);
+at::Tensor fp4_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_sf,
+                      const c10::optional<at::Tensor>& w_row, int64_t parts, int64_t fmt,
+                      const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
+                      const at::Tensor& status);
+at::Tensor fp4_linear_dgrad(const at::Tensor& dy, const at::Tensor& w, const at::Tensor& w_sf,
+                            const c10::optional<at::Tensor>& w_row, int64_t parts, int64_t K, int64_t fmt,
+                            const at::Tensor& status);
+at::Tensor fp4_ffn(const at::Tensor& x, const at::Tensor& gu, const at::Tensor& gu_sf,
+                   const c10::optional<at::Tensor>& gu_row, int64_t gu_fmt, const at::Tensor& dn, const at::Tensor& dn_sf,
+                   const c10::optional<at::Tensor>& dn_row, int64_t dn_fmt, int64_t act,
+                   const c10::optional<at::Tensor>& gu_bias, const c10::optional<at::Tensor>& dn_bias,
+                   const c10::optional<at::Tensor>& residual, const at::Tensor& status);
 void sharded_grad_reduce(const at::Tensor& grad_ptrs, int64_t world, int64_t off, int64_t n, at::Tensor& shard,
                          at::Tensor& norm_sq);
 void sharded_adamw(const at::Tensor& shard_grad, int64_t off, int64_t n, const at::Tensor& master_ptrs,
@@ -211,7 +232,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("few_rows_linear", &rx::few_rows_linear, "bf16 (gated) projection of 1 to 64 token rows");
   m.def("fp4_quantize", &rx::fp4_quantize, "MXFP4 / NVFP4 quantiser");
   m.def("fp4_dequantize", &rx::fp4_dequantize, "values of MXFP4 / NVFP4 codes and scales");
-  m.def("fp4_gemm", &rx::fp4_gemm, "tcgen05 block-scaled 4-bit GEMM, plain or gated");
+  m.def("gated_ffn_forward", &rx::gated_ffn_forward, "forward of the gated feed-forward block");
+  m.def("gated_ffn_backward", &rx::gated_ffn_backward, "gradients of the gated feed-forward block");
+  m.def("fp4_gemm", &rx::fp4_gemm, "tcgen05 block-scaled 4-bit GEMM");
+  m.def("fp4_linear", &rx::fp4_linear, "linear layer: activations quantised to 4 bits, 4-bit weight");
+  m.def("fp4_linear_dgrad", &rx::fp4_linear_dgrad, "input gradient of the 4-bit linear layer");
+  m.def("fp4_ffn", &rx::fp4_ffn, "gated feed-forward block over 4-bit operands");
   m.def("mnr_tc_argmax", &rx::mnr_tc_argmax, "tcgen05 split-bf16 scores reduced to each row's hardest candidate");
   m.def("sharded_grad_reduce", &rx::sharded_grad_reduce);
   m.def("sharded_adamw", &rx::sharded_adamw);

@@ -63,6 +63,15 @@ inline EncodeTiledFn encode_tiled_fn() {
              "cuTensorMapEncodeTiled is unavailable");
     fn = reinterpret_cast<EncodeTiledFn>(raw);
   }
+  // The driver call needs a current context, which a thread that has not launched anything yet
+  // (an autograd worker whose first work is one of these kernels) does not have.
+  static thread_local bool bound = false;
+  if (!bound) {
+    int device = 0;
+    RX_CUDA_CHECK(cudaGetDevice(&device));
+    RX_CUDA_CHECK(cudaSetDevice(device));
+    bound = true;
+  }
   return fn;
 }
 

@@ -10,14 +10,17 @@
 // twice over; each CTA streams its share of W through a TMA ring (about 100 KB,
 // two CTAs per SM) into fp32 TMEM accumulators. The partial sums meet in
 // shared memory: after a cluster barrier every warp of the cluster takes
-// groups of 32 outputs, reads the partials of all CTAs through distributed
-// shared memory in rank order (so results do not depend on timing) and runs the
-// epilogue.
+// a token's 128 outputs, adds the partials of all CTAs, read through
+// distributed shared memory, in rank order (so results do not depend on timing)
+// and runs the epilogue.
 //
 // A gated tile has two accumulators, 128 gate rows and the 128 up rows of the
 // same output columns, so one lane holds both operands of the product. With
-// `q_out` the products leave as MXFP4: the 32 outputs of a warp's group are one
-// scale block.
+// `q_out` the products leave as MXFP4, eight lanes to a scale block.
+//
+// W does not depend on the kernel that produces x. Where the host says that
+// kernel is the one just before (`after_producer`), this one is launched
+// early: it fills its ring with W and waits for x only then.
 //
 // Bound by HBM: floor = bytes of W / copy bandwidth. Every wait is bounded.
 #include "few_rows.h"
@@ -53,9 +56,10 @@ struct Shape {
   static_assert(kStages >= 2 && kCols <= 256, "two CTAs per SM must fit");
 };
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+// Four consecutive floats of another CTA's shared memory.
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
 }
 
@@ -77,7 +81,32 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * rank / splits);
   const int kb1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (rank + 1) / splits);
 
+  // The weight tiles (and scales) of K block kb into stage s; the token tile follows in load_x.
+  auto load_w = [&](int kb, int s) {
+    mbar_arrive_expect_tx(&full[s], S::kTiles + S::kSfW + S::kSfX);
+    uint8_t* dst = base + s * S::kStage;
+    const int x = kb * (KIND == kBf16 ? 64 : 128);  // tensor-map column of the stage (elements of the map)
+#pragma unroll
+    for (int b = 0; b < PARTS; ++b) tma_load_2d(dst + b * kTileW, &tmW, &full[s], x, tile * 128 + b * p.N);
+    if constexpr (KIND != kBf16) {
+      const int64_t row_tiles = (p.N + 127) >> 7, g = static_cast<int64_t>(kb) * S::kGroups;
+#pragma unroll
+      for (int b = 0; b < PARTS; ++b)
+        bulk_load(dst + S::kTiles + b * S::kGroups * 512, p.sf_w + ((tile + b * row_tiles) * p.groups + g) * 512,
+                  S::kGroups * 512, &full[s]);
+    }
+  };
+  auto load_x = [&](int kb, int s) {
+    uint8_t* dst = base + s * S::kStage;
+    tma_load_2d(dst + PARTS * kTileW, &tmX, &full[s], kb * (KIND == kBf16 ? 64 : 128), 0);
+    if constexpr (KIND != kBf16)
+      bulk_load(dst + S::kTiles + S::kSfW, p.sf_x + static_cast<int64_t>(kb) * S::kGroups * 512, S::kSfX, &full[s]);
+  };
+
+  const int first = min(S::kStages, kb1 - kb0);  // K blocks that fill the empty ring
   if (threadIdx.x == 0) {
+    tma_prefetch_map(&tmW);
+    tma_prefetch_map(&tmX);
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -85,6 +114,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_mbarrier_init();
+    for (int i = 0; i < first; ++i) load_w(kb0 + i, i);  // W does not depend on the kernel before
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, S::kTmemCols);
@@ -93,36 +123,26 @@ __global__ void __launch_bounds__(kThreads, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  grid_launch_dependents();
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
+      grid_dependency_wait();
       uint32_t issued = 0, parity = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
         const int i = kb - kb0, s = i % S::kStages;
         const uint32_t phase = (i / S::kStages) & 1;
-        if (*abort_flag || !mbar_wait(&empty[s], phase ^ 1, p.timeout_ns)) {
-          report_status(p.status, kStatusTimeoutProducer);
-          *abort_flag = 1;
-          break;
+        if (i >= first) {
+          if (*abort_flag || !mbar_wait(&empty[s], phase ^ 1, p.timeout_ns)) {
+            report_status(p.status, kStatusTimeoutProducer);
+            *abort_flag = 1;
+            break;
+          }
+          load_w(kb, s);
         }
-        mbar_arrive_expect_tx(&full[s], S::kTiles + S::kSfW + S::kSfX);
-        uint8_t* dst = base + s * S::kStage;
-        const int x = kb * (KIND == kBf16 ? 64 : 128);  // tensor-map column of the stage (elements of the map)
-#pragma unroll
-        for (int b = 0; b < PARTS; ++b) tma_load_2d(dst + b * kTileW, &tmW, &full[s], x, tile * 128 + b * p.N);
-        tma_load_2d(dst + PARTS * kTileW, &tmX, &full[s], x, 0);
-        if constexpr (KIND != kBf16) {
-          uint8_t* sf = dst + S::kTiles;
-          const int64_t row_tiles = (p.N + 127) >> 7;
-          const int64_t g = static_cast<int64_t>(kb) * S::kGroups;
-#pragma unroll
-          for (int b = 0; b < PARTS; ++b)
-            bulk_load(sf + b * S::kGroups * 512, p.sf_w + ((tile + b * row_tiles) * p.groups + g) * 512, S::kGroups * 512,
-                      &full[s]);
-          bulk_load(sf + S::kSfW, p.sf_x + g * 512, S::kSfX, &full[s]);
-        }
+        load_x(kb, s);
         issued |= 1u << s;
         parity = (parity & ~(1u << s)) | (phase << s);
       }
@@ -205,52 +225,82 @@ __global__ void __launch_bounds__(kThreads, 2)
   cluster_sync_all();
 
   // ------------------------------------------------------------ reduction and epilogue
-  // Group g: token t = g / 4, the 32 output columns (g % 4) of the tile.
-  const uint32_t part_addr = smem_u32(part);
-  const bool aborted = *abort_flag != 0;
-  if (!aborted) {
-    for (int g = rank * kWarps + warp; g < p.T * 4; g += splits * kWarps) {
-      const int t = g >> 2, col = (g & 3) * 32 + lane;
-      const int n = tile * 128 + col;
-      float v[PARTS];
+  // A warp takes a token's 128 columns of the tile, a lane four of them.
+  grid_dependency_wait();
+  const uint32_t part_addr = smem_u32(part) + lane * 16;
+  const int n = tile * 128 + lane * 4;
+  if (*abort_flag == 0) {
+    for (int t = rank * kWarps + warp; t < p.T; t += splits * kWarps) {
+      float4 in[PARTS][8];
 #pragma unroll
-      for (int b = 0; b < PARTS; ++b) v[b] = 0.f;
-      for (int r = 0; r < splits; ++r) {
-        const uint32_t peer = mapa_shared(part_addr, static_cast<uint32_t>(r));
+      for (int r = 0; r < 8; ++r) {
+        if (r < splits) {
+          const uint32_t peer = mapa_shared(part_addr, static_cast<uint32_t>(r));
 #pragma unroll
-        for (int b = 0; b < PARTS; ++b) v[b] += ld_cluster_f32(peer + ((b * NT + t) * kPartLd + col) * 4);
-      }
-      const bool live = n < p.N;
-      if (live) {
-#pragma unroll
-        for (int b = 0; b < PARTS; ++b) {
-          if constexpr (KIND == kNvfp4) v[b] *= p.row_x[t] * p.row_w[static_cast<int64_t>(b) * p.N + n];
-          if (p.bias != nullptr) v[b] += __bfloat162float(p.bias[static_cast<int64_t>(b) * p.N + n]);
+          for (int b = 0; b < PARTS; ++b) in[b][r] = ld_cluster_f4(peer + (b * NT + t) * kPartLd * 4);
         }
       }
-      float y = v[0];
-      if constexpr (PARTS == 2) y = gated::act_value(v[0], p.act) * v[1];
-      if constexpr (PARTS == 1)
-        if (live && p.residual != nullptr) y += __bfloat162float(p.residual[static_cast<int64_t>(t) * p.ld_res + n]);
+      float v[PARTS][4];
+#pragma unroll
+      for (int b = 0; b < PARTS; ++b) {
+        v[b][0] = v[b][1] = v[b][2] = v[b][3] = 0.f;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          if (r < splits) {
+            v[b][0] += in[b][r].x;
+            v[b][1] += in[b][r].y;
+            v[b][2] += in[b][r].z;
+            v[b][3] += in[b][r].w;
+          }
+        }
+        const int64_t c0 = static_cast<int64_t>(b) * p.N + n;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (n + j < p.N) {
+            if constexpr (KIND == kNvfp4) v[b][j] *= p.row_x[t] * p.row_w[c0 + j];
+            if (p.bias != nullptr) v[b][j] += __bfloat162float(p.bias[c0 + j]);
+          }
+        }
+      }
+      float y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        y[j] = v[0][j];
+        if constexpr (PARTS == 2) y[j] = gated::act_value(v[0][j], p.act) * v[1][j];
+        if constexpr (PARTS == 1)
+          if (n + j < p.N && p.residual != nullptr) y[j] += __bfloat162float(p.residual[t * p.ld_res + n + j]);
+      }
       if constexpr (PARTS == 2 && KIND == kMxfp4) {
-        if (p.q_out != nullptr) {
-          if (!live) y = 0.f;
-          uint32_t top = __float_as_uint(y) & 0x7fffffffu;
+        if (p.q_out != nullptr) {  // eight lanes hold a block of 32
+          uint32_t top = 0;
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          for (int j = 0; j < 4; ++j) {
+            if (n + j >= p.N) y[j] = 0.f;
+            top = max(top, __float_as_uint(y[j]) & 0x7fffffffu);
+          }
+#pragma unroll
+          for (int o = 1; o < 8; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
           const uint32_t byte = fp4::mx_scale_byte(top);
-          y *= fp4::mx_inverse(byte);
-          float w8[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) w8[j] = __shfl_sync(0xffffffffu, y, (lane & 24) + j);
-          const uint32_t codes = fp4::pack8(w8);
-          const int64_t at = static_cast<int64_t>(t) * p.ld_q + (n >> 1);
-          if ((lane & 7) == 0 && (n >> 1) + 4 <= p.ld_q) *reinterpret_cast<uint32_t*>(p.q_out + at) = codes;
-          if (lane == 0) p.q_sf[fp4::scale_offset(t, n >> 5, p.q_groups)] = static_cast<uint8_t>(byte);
+          const float inv = fp4::mx_inverse(byte);
+          const float w8[8] = {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv, 0.f, 0.f, 0.f, 0.f};
+          if ((n >> 1) < p.ld_q)
+            *reinterpret_cast<uint16_t*>(p.q_out + t * p.ld_q + (n >> 1)) = static_cast<uint16_t>(fp4::pack8(w8));
+          if ((lane & 7) == 0) p.q_sf[fp4::scale_offset(t, n >> 5, p.q_groups)] = static_cast<uint8_t>(byte);
           continue;
         }
       }
-      if (live) p.out[static_cast<int64_t>(t) * p.ld_out + n] = __float2bfloat16_rn(y);
+      __nv_bfloat16* out = p.out + t * p.ld_out + n;
+      if (p.vec && n + 4 <= p.N) {
+        uint2 w;
+        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
+        h[0] = __floats2bfloat162_rn(y[0], y[1]);
+        h[1] = __floats2bfloat162_rn(y[2], y[3]);
+        *reinterpret_cast<uint2*>(out) = w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.N) out[j] = __float2bfloat16_rn(y[j]);
+      }
     }
   }
   tc_fence_before();
@@ -278,13 +328,15 @@ cudaError_t launch_shape(const CUtensorMap& map_x, const CUtensorMap& map_w, con
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1;
   attr[0].val.clusterDim.y = splits;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = p.after_producer ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, map_x, map_w, p);
 }
 

@@ -22,6 +22,7 @@ struct Params {
   int64_t ld_res;
   __nv_bfloat16* out;             // [T, N], or null with q_out
   int64_t ld_out;
+  int vec;                        // rows of out are 8-byte aligned
   // 4-bit operands
   const uint8_t* sf_x;
   const uint8_t* sf_w;
@@ -33,6 +34,9 @@ struct Params {
   int64_t ld_q;
   uint8_t* q_sf;
   int64_t q_groups;
+  // The kernel before this one in the stream writes x (and nothing else that this one reads) and
+  // lets dependents start early: stream W before it has finished.
+  int after_producer;
   int* status;
   uint64_t timeout_ns;
 };

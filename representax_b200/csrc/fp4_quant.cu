@@ -12,11 +12,16 @@
 // and products are NaN.
 //
 // Bound by HBM: x is read once (2 or 4 bytes a value), half a byte a value and
-// the scales are written. A lane takes 8 consecutive values (one or two 16-byte
-// loads, one 4-byte store), so a warp covers 256 consecutive ones and a
-// block's maximum needs one or two shuffles. A row belongs to 1, 2, 4 or 8 warps
-// by its length; NVFP4 keeps up to 8 x kKeep values a lane in registers between the
-// row's maximum and the codes and reads longer rows a second time.
+// the scales are written; the instructions per value are the next limit, so
+//  * a lane takes 8 consecutive values (one or two 16-byte loads, one 4-byte
+//    store) and a warp 256; maxima are taken on the raw 16-bit pairs;
+//  * a warp has up to kKeep such pieces of its row in flight and keeps them
+//    in registers, so NVFP4 has the row's maximum before it codes without a
+//    second read (rows beyond 8 warps * kKeep pieces are read twice);
+//  * a quotient by an E4M3 scale is a product with its reciprocal and one
+//    correction step (Markstein, "Computation of elementary functions on the
+//    IBM RISC System/6000 processor", 1990): the correctly rounded quotient
+//    in three operations, so ties fall as the definition says.
 #include "fp4.h"
 
 #include <cuda_fp16.h>
@@ -28,7 +33,10 @@ namespace rx {
 namespace fp4 {
 
 constexpr int kQuantThreads = 256;
-constexpr int kKeep = 4;
+constexpr int kQuantWarps = kQuantThreads / 32;
+// Pieces of 256 values that a warp keeps in registers.
+template <typename T, int FMT>
+constexpr int kKeep = (FMT == kMx ? 8 : 16) / sizeof(T);
 
 template <typename T>
 __device__ __forceinline__ float to_float(T v) { return static_cast<float>(v); }
@@ -44,29 +52,68 @@ __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bf
 template <>
 __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 
-// Eight consecutive values of a row from column c, zeros past K.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int c, int K, float (&v)[8]) {
-  if (VEC && c + 8 <= K) {
-    constexpr int kLoads = sizeof(T) / 2;
-    uint4 w[kLoads];
+// Eight consecutive values as loaded: four 32-bit words of 16-bit pairs, or eight fp32 words.
+template <typename T>
+struct Raw {
+  static constexpr int kWords = 2 * sizeof(T);
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) w[i] = ldg_v4_issue(reinterpret_cast<const uint4*>(row + c) + i);
+    for (int i = 0; i < kWords; ++i) w[i] = 0u;
+  }
+  // Columns c.. of a row, zeros past K.
+  template <bool VEC>
+  __device__ __forceinline__ void load(const T* row, int c, int K) {
+    if (VEC && c + 8 <= K) {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 v = ldg_v4_issue(reinterpret_cast<const uint4*>(row + c) + i);
+        w[4 * i] = v.x;
+        w[4 * i + 1] = v.y;
+        w[4 * i + 2] = v.z;
+        w[4 * i + 3] = v.w;
+      }
+    } else {
+      zero();
+      T* e = reinterpret_cast<T*>(w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < K) e[i] = row[c + i];
+    }
+  }
+  // Bits of the largest magnitude, comparable as integers (NaN above infinity above finite
+  // values): in each half of the word for 16-bit types.
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t t = 0;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 2)
+        t = __vmaxu2(t, w[i] & 0x7fff7fffu);
+      else
+        t = max(t, w[i] & 0x7fffffffu);
+    }
+    return t;
+  }
+  // Float bits of a magnitude from top().
+  static __device__ __forceinline__ uint32_t top_bits(uint32_t t) {
+    if constexpr (sizeof(T) == 4) return t;
+    const uint32_t m = max(t & 0xffffu, t >> 16);
+    if constexpr (sizeof(T) == 2) {
+      const unsigned short h = static_cast<unsigned short>(m);
+      return __float_as_uint(to_float(*reinterpret_cast<const T*>(&h))) & 0x7fffffffu;
+    }
+    return m;
+  }
+  static __device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b) {
+    return sizeof(T) == 2 ? __vmaxu2(a, b) : max(a, b);
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
     const T* e = reinterpret_cast<const T*>(w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = to_float(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < K ? to_float(row[c + i]) : 0.f;
   }
-}
-
-__device__ __forceinline__ uint32_t top8(const float (&v)[8]) {
-  uint32_t t = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) t = max(t, __float_as_uint(v[i]) & 0x7fffffffu);
-  return t;
-}
+};
 
 // 2^ceil(log2(top / 2688)) from the float bits of the row's largest magnitude.
 __device__ __forceinline__ float row_factor(uint32_t top) {
@@ -80,75 +127,83 @@ __device__ __forceinline__ float e4m3_value(uint32_t byte) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
 }
 
-// Rows of a CTA: kQuantThreads / (32 * warps_per_row). Every warp of a row walks
-// the padded extent groups * (values of a group) in steps of 256 values, so all
-// scale bytes of the row tiles, padding included, are written.
+// A row belongs to `warps_per_row` warps (1, 2, 4 or 8); piece i of a warp is the
+// 256 values from (i * warps_per_row + its place in the row) * 256. Every warp walks
+// the padded extent, so all scale bytes of the row tiles are written.
 template <typename T, int FMT, bool VEC>
-__global__ void __launch_bounds__(kQuantThreads)
-    quantize_kernel(const QuantParams p, int warps_per_row) {
-  __shared__ uint32_t tops[kQuantThreads / 32];
+__global__ void __launch_bounds__(kQuantThreads, FMT == kMx ? 4 : 2) quantize_kernel(const QuantParams p, int warps_per_row) {
+  __shared__ uint32_t tops[kQuantWarps];
+  grid_launch_dependents();  // a product of these codes may fetch its other operand meanwhile
   const int warp = warp_id(), lane = lane_id();
-  const int rows_per_cta = (kQuantThreads / 32) / warps_per_row;
-  const int part_of_row = warp % warps_per_row;
+  const int rows_per_cta = kQuantWarps / warps_per_row;
+  const int place = warp % warps_per_row;
   const int64_t padded = (p.rows + 127) / 128 * 128;
   const int64_t slot = static_cast<int64_t>(blockIdx.x) * rows_per_cta + warp / warps_per_row;  // row of the padded tiles
-  const int64_t part = slot / padded, r = slot % padded;
-  const bool in_grid = part < p.parts, live = in_grid && r < p.rows;
+  const int64_t part = p.parts == 1 ? 0 : slot / padded;
+  const int64_t r = slot - part * padded;
+  const bool in_grid = slot < p.parts * padded, live = in_grid && r < p.rows;
   const int64_t row = part * p.rows + r;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const int extent = static_cast<int>(p.groups) * 4 * block_of(FMT);
-  const int c0 = part_of_row * 256 + lane * 8, step = warps_per_row * 256;
-  const int64_t sf_row = part * padded + r;
+  const int step = warps_per_row * 256;
+  const int p0 = place * 256 + blockIdx.y * kKeep<T, FMT> * step;  // first column of the warp (grid.y is 1 in NVFP4)
+  const int c0 = p0 + lane * 8;
+  const int K = live ? p.K : 0;  // rows of the padding hold nothing
 
-  float factor = 1.f;
-  float keep[FMT == kNv ? kKeep : 1][8];
-  if constexpr (FMT == kNv) {
-    uint32_t top = 0;
-    if (live) {
+  Raw<T> raw[kKeep<T, FMT>];
 #pragma unroll
-      for (int i = 0; i < kKeep; ++i) {
-        if (c0 + i * step < p.K) {
-          load8<T, VEC>(x, c0 + i * step, p.K, keep[i]);
-          top = max(top, top8(keep[i]));
-        }
-      }
-      for (int c = c0 + kKeep * step; c < p.K; c += step) {
-        float v[8];
-        load8<T, VEC>(x, c, p.K, v);
-        top = max(top, top8(v));
-      }
+  for (int i = 0; i < kKeep<T, FMT>; ++i) {
+    raw[i].zero();
+    if (c0 + i * step < K) raw[i].template load<VEC>(x, c0 + i * step, K);
+  }
+  float factor = 1.f, inv_factor = 1.f;
+  if constexpr (FMT == kNv) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int i = 0; i < kKeep<T, FMT>; ++i) t = Raw<T>::max_of(t, raw[i].top());
+    for (int c = c0 + kKeep<T, FMT> * step; c < K; c += step) {
+      Raw<T> v;
+      v.template load<VEC>(x, c, K);
+      t = Raw<T>::max_of(t, v.top());
     }
-    top = __reduce_max_sync(0xffffffffu, top);
+    uint32_t top = __reduce_max_sync(0xffffffffu, Raw<T>::top_bits(t));
     if (warps_per_row > 1) {  // the same for every thread of the CTA
       if (lane == 0) tops[warp] = top;
       __syncthreads();
-      for (int i = 0; i < warps_per_row; ++i) top = max(top, tops[warp - part_of_row + i]);
+      for (int i = 0; i < warps_per_row; ++i) top = max(top, tops[warp - place + i]);
     }
     factor = row_factor(top);
-    if (live && part_of_row == 0 && lane == 0) p.row_scale[row] = factor;
+    inv_factor = __uint_as_float(0x7f000000u - __float_as_uint(factor));  // 2^-e (any value for a NaN factor)
+    if (live && place == 0 && lane == 0) p.row_scale[row] = factor;
   }
   if (!in_grid) return;
 
-  auto emit = [&](const float (&v)[8], int c) {
-    uint32_t top = top8(v);
-    uint32_t byte, codes;
-    float w[8];
+  const int64_t sf_row = part * padded + r;
+  uint8_t* sf = p.sf + scale_offset(sf_row, 0, p.groups);
+  uint8_t* q = p.q + row * p.ldq;
+  auto emit = [&](const Raw<T>& in, int c) {
+    uint32_t t = in.top(), byte;
+    float v[8];
+    in.values(v);
+    t = Raw<T>::max_of(t, __shfl_xor_sync(0xffffffffu, t, 1));
     if constexpr (FMT == kMx) {
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      byte = mx_scale_byte(top);
+      t = Raw<T>::max_of(t, __shfl_xor_sync(0xffffffffu, t, 2));
+      byte = mx_scale_byte(Raw<T>::top_bits(t));
       const float inv = mx_inverse(byte);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = v[i] * inv;
+      for (int i = 0; i < 8; ++i) v[i] *= inv;
     } else {
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      const float want = __fdiv_rn(__fdiv_rn(__uint_as_float(top), 6.f), factor);
+      const float want = __fdiv_rn(__uint_as_float(Raw<T>::top_bits(t)), 6.f) * inv_factor;
       byte = __nv_cvt_float_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
-      const float scale = e4m3_value(byte) * factor;
+      // a row with a NaN factor is NaN by that factor whatever its codes; a zero scale has zero codes
+      const float s = e4m3_value(byte), inv = s > 0.f ? __frcp_rn(s) : 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = scale > 0.f ? __fdiv_rn(v[i], scale) : 0.f;
+      for (int i = 0; i < 8; ++i) {
+        const float a = v[i] * inv_factor, guess = a * inv;
+        v[i] = fmaf(fmaf(-guess, s, a), inv, guess);
+      }
     }
-    codes = pack8(w);
+    const uint32_t codes = pack8(v);
     // four blocks' bytes -> one 4-byte word of the group, written by its first lane
     constexpr int kLanes = block_of(FMT) / 8;  // lanes of a block
     uint32_t word = byte << (8 * ((lane / kLanes) & 3));
@@ -156,46 +211,44 @@ __global__ void __launch_bounds__(kQuantThreads)
     for (int o = kLanes; o < 4 * kLanes; o *= 2) word |= __shfl_xor_sync(0xffffffffu, word, o);
     if (c < extent) {
       if (lane % (4 * kLanes) == 0)
-        *reinterpret_cast<uint32_t*>(p.sf + scale_offset(sf_row, c / block_of(FMT), p.groups)) = live ? word : 0u;
-      if (live && (c >> 1) < p.ldq) *reinterpret_cast<uint32_t*>(p.q + row * p.ldq + (c >> 1)) = codes;
+        *reinterpret_cast<uint32_t*>(sf + static_cast<int64_t>(c / (4 * block_of(FMT))) * 512) = live ? word : 0u;
+      if (live && (c >> 1) < p.ldq) *reinterpret_cast<uint32_t*>(q + (c >> 1)) = codes;
     }
   };
-
-  int i = 0;
-  for (int c = c0; c - lane * 8 < extent; c += step, ++i) {  // warp-uniform
-    float v[8];
-    if constexpr (FMT == kNv) {
-      if (i < kKeep) {
 #pragma unroll
-        for (int j = 0; j < kKeep; ++j)
-          if (j == i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = live && c < p.K ? keep[j][e] : 0.f;
-        emit(v, c);
-        continue;
-      }
-    }
-    if (live && c < p.K) {
-      load8<T, VEC>(x, c, p.K, v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
-    }
-    emit(v, c);
+  for (int i = 0; i < kKeep<T, FMT>; ++i) {
+    if (p0 + i * step < extent) emit(raw[i], c0 + i * step);  // warp-uniform
   }
+  if constexpr (FMT == kNv) {
+    for (int c = c0 + kKeep<T, FMT> * step; c - lane * 8 < extent; c += step) {
+      Raw<T> v;
+      v.zero();
+      if (c < K) v.template load<VEC>(x, c, K);
+      emit(v, c);
+    }
+  }
+}
+
+// Warps of a row: enough that a warp keeps its whole share in registers, more while the rows are too few to
+// give every SM 16 warps.
+static int row_warps(int64_t slots, int64_t pieces, int keep) {
+  int wpr = 1;
+  while (wpr < kQuantWarps && (pieces > static_cast<int64_t>(wpr) * keep || (wpr < pieces && slots * wpr < 148 * 16))) wpr *= 2;
+  return wpr;
 }
 
 template <typename T, int FMT>
 cudaError_t quantize_typed(const QuantParams& p, cudaStream_t stream) {
   const bool vec = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.ldx % (16 / sizeof(T)) == 0;
-  const int64_t chunks = (p.K + 255) / 256;
-  const int wpr = chunks <= 1 ? 1 : (chunks <= 2 ? 2 : (chunks <= 4 ? 4 : 8));
   const int64_t slots = p.parts * ((p.rows + 127) / 128 * 128);
-  const int64_t grid = (slots * wpr + kQuantThreads / 32 - 1) / (kQuantThreads / 32);
+  const int wpr = row_warps(slots, (p.K + 255) / 256, kKeep<T, FMT>);
+  const int64_t extent = p.groups * 4 * block_of(FMT), share = static_cast<int64_t>(wpr) * kKeep<T, FMT> * 256;
+  const dim3 grid(static_cast<unsigned>((slots * wpr + kQuantWarps - 1) / kQuantWarps),
+                  FMT == kMx ? static_cast<unsigned>((extent + share - 1) / share) : 1u);
   if (vec)
-    quantize_kernel<T, FMT, true><<<static_cast<unsigned>(grid), kQuantThreads, 0, stream>>>(p, wpr);
+    quantize_kernel<T, FMT, true><<<grid, kQuantThreads, 0, stream>>>(p, wpr);
   else
-    quantize_kernel<T, FMT, false><<<static_cast<unsigned>(grid), kQuantThreads, 0, stream>>>(p, wpr);
+    quantize_kernel<T, FMT, false><<<grid, kQuantThreads, 0, stream>>>(p, wpr);
   return cudaGetLastError();
 }
 
@@ -208,41 +261,44 @@ cudaError_t quantize(const QuantParams& p, int fmt, int type, cudaStream_t strea
   }
 }
 
-// One thread: 8 values of a row.
+// Lane: 16 bytes of output (8 or 4 consecutive values) per piece, so a warp stores 512 contiguous bytes.
 template <typename T, int FMT>
-__global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams p, bool vec) {
-  const int64_t padded = (p.rows + 127) / 128 * 128;
-  const int per_row = (p.K + 7) / 8;
-  const int64_t total = p.parts * p.rows * per_row;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t row = i / per_row;
-    const int c = static_cast<int>(i - row * per_row) * 8;
-    const int64_t part = row / p.rows;
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(p.q + row * p.ldq + (c >> 1));
-    const uint32_t byte = p.sf[scale_offset(part * padded + row - part * p.rows, c / block_of(FMT), p.groups)];
+__global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const DequantParams p, int warps_per_row, bool vec) {
+  constexpr int kVals = 16 / sizeof(T), kPiece = 32 * kVals;
+  const int warp = warp_id(), lane = lane_id();
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kQuantWarps / warps_per_row) + warp / warps_per_row;
+  if (row >= p.parts * p.rows) return;
+  const int64_t part = p.parts == 1 ? 0 : row / p.rows;
+  const uint8_t* sf = p.sf + scale_offset(part * ((p.rows + 127) / 128 * 128) + row - part * p.rows, 0, p.groups);
+  const uint8_t* q = p.q + row * p.ldq;
+  const float factor = FMT == kNv ? p.row_scale[row] : 1.f;
+  T* out = static_cast<T*>(p.out) + row * p.ldo;
+#pragma unroll 4
+  for (int c = (warp % warps_per_row) * kPiece + lane * kVals; c < p.K; c += warps_per_row * kPiece) {
+    const uint32_t codes = kVals == 8 ? *reinterpret_cast<const uint32_t*>(q + (c >> 1))
+                                      : *reinterpret_cast<const uint16_t*>(q + (c >> 1));
+    const int block = c / block_of(FMT);
+    const uint32_t byte = sf[static_cast<int64_t>(block >> 2) * 512 + (block & 3)];
     float scale;
     if constexpr (FMT == kMx)
       scale = byte == 0xffu ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
     else
-      scale = e4m3_value(byte) * p.row_scale[row];
-    T v[8];
+      scale = e4m3_value(byte) * factor;
+    T v[kVals];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < kVals; ++j) {
       const uint32_t n = (codes >> (4 * j)) & 0xfu;
       // magnitude codes 0..7: 0, 0.5, then (1 + m / 2) 2^(e - 1)
       const uint32_t mag = n & 7u;
       const float m = mag < 2u ? 0.5f * mag : __uint_as_float(((mag >> 1) + 126u) << 23 | (mag & 1u) << 22);
       v[j] = from_float<T>((n & 8u ? -m : m) * scale);
     }
-    T* dst = static_cast<T*>(p.out) + row * p.ldo + c;
-    if (vec && c + 8 <= p.K) {
-      constexpr int kStores = sizeof(T) / 2;
-      const uint4* w = reinterpret_cast<const uint4*>(v);
-#pragma unroll
-      for (int j = 0; j < kStores; ++j) reinterpret_cast<uint4*>(dst)[j] = w[j];
+    if (vec && c + kVals <= p.K) {
+      *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<const uint4*>(v);
     } else {
-      for (int j = 0; j < 8 && c + j < p.K; ++j) dst[j] = v[j];
+#pragma unroll
+      for (int j = 0; j < kVals; ++j)
+        if (c + j < p.K) out[c + j] = v[j];
     }
   }
 }
@@ -250,13 +306,13 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams p, 
 template <typename T>
 cudaError_t dequantize_typed(const DequantParams& p, int fmt, cudaStream_t stream) {
   const bool vec = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo % (16 / sizeof(T)) == 0;
-  const int64_t total = p.parts * p.rows * ((p.K + 7) / 8);
-  const int64_t want = (total + 255) / 256;
-  const unsigned grid = static_cast<unsigned>(want < 148 * 32 ? want : 148 * 32);
+  const int64_t rows = p.parts * p.rows;
+  const int wpr = row_warps(rows, (p.K + 512 / static_cast<int>(sizeof(T)) - 1) / (512 / static_cast<int>(sizeof(T))), 16);
+  const unsigned grid = static_cast<unsigned>((rows * wpr + kQuantWarps - 1) / kQuantWarps);
   if (fmt == kMx)
-    dequantize_kernel<T, kMx><<<grid, 256, 0, stream>>>(p, vec);
+    dequantize_kernel<T, kMx><<<grid, kQuantThreads, 0, stream>>>(p, wpr, vec);
   else
-    dequantize_kernel<T, kNv><<<grid, 256, 0, stream>>>(p, vec);
+    dequantize_kernel<T, kNv><<<grid, kQuantThreads, 0, stream>>>(p, wpr, vec);
   return cudaGetLastError();
 }
 

@@ -29,40 +29,28 @@
 // host entries). The main loops follow the pair kernel of gemm_kernel.cuh: six
 // 32 KB stages, TMA with the 128-byte swizzle, one issuing thread, two
 // accumulator buffers so that an epilogue overlaps the next tile's products.
+#include "gated.h"
+
 #include <cuda_fp16.h>
 
 #include <algorithm>
 
 #include "gated_act.cuh"
-#include "gemm_kernel.cuh"
+#include "sm100.cuh"
+#include "tile_io.cuh"
 
 namespace rx {
 namespace gated {
 
-using gemm::BK;
-using gemm::BM;
-using gemm::kEpilogueWarps;
-using gemm::kThreads;
+constexpr int BM = 128, BK = 64;
+constexpr int kEpilogueWarps = 8;  // two per TMEM lane quadrant, each owning half the columns
+constexpr int kThreads = 64 + 32 * kEpilogueWarps;
 
 constexpr int kStages = 6;
 constexpr int kTile = BM * BK * 2;  // 16 KB: 128 rows x 64 bf16
 constexpr int kStaging = kEpilogueWarps * 2 * 2048;
 constexpr size_t kSmem = 1024 + kStages * 2 * kTile + kStaging + 256;
 static_assert(kSmem <= 232448, "shared memory beyond the opt-in limit");
-
-struct Params {
-  int M, N, K;  // N: columns of h (forward) or of dh (backward)
-  int m_tiles, n_tiles, num_units;
-  int act;
-  const __nv_bfloat16* bias;  // forward: [2 N] (gate, up) or null
-  const __half* saved_b;      // backward: b [M, N], a [M, N] with row stride ld_saved
-  const __half* saved_a;
-  int64_t ld_saved;
-  uint16_t* exps;             // [M, ceil(N / 32)]: low byte the block exponent of b, high byte that of a
-  int64_t ld_exps;
-  int* status;
-  uint64_t timeout_ns;
-};
 
 // Exponent byte e of a block with largest magnitude `top`: values are stored
 // times 2^(141 - e) and read back times 2^(e - 141). Clamped so that both
@@ -130,15 +118,14 @@ __device__ __forceinline__ void add_bias32(const __nv_bfloat16* bias, int n_base
   }
 }
 
-// MODE 0: forward; 1: forward that saves a and b; 2: backward (dz).
 template <int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
     gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmOut0, const __grid_constant__ CUtensorMap tmOut1,
                  const __grid_constant__ CUtensorMap tmOut2, const Params p) {
-  constexpr bool kBackward = MODE == 2;
-  constexpr bool kSave = MODE == 1;
-  constexpr int kTileCols = kBackward ? 256 : 128;  // output columns of a tile
+  constexpr bool kDz = MODE == kBackward;
+  constexpr bool kSave = MODE == kForwardSave;
+  constexpr int kTileCols = kDz ? 256 : 128;  // output columns of a tile
   constexpr uint32_t kTmemCols = 512;
 
   extern __shared__ uint8_t smem_raw[];
@@ -209,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint8_t* a_dst = sA + stage * kTile;
           uint8_t* b_dst = sB + stage * kTile;
           tma_load_2d_pair(a_dst, &tmA, bar, kb * BK, m);
-          if constexpr (kBackward) {  // Wd [K, N] is MN-major: two 64 x 64 boxes
+          if constexpr (kDz) {  // Wd [K, N] is MN-major: two 64 x 64 boxes
             tma_load_2d_pair(b_dst, &tmB, bar, n0 + rank * 128, kb * BK);
             tma_load_2d_pair(b_dst + 8192, &tmB, bar, n0 + rank * 128 + 64, kb * BK);
           } else {  // CTA 0: gate rows, CTA 1: up rows of the same columns
@@ -236,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (even CTA)
     if (leader && lane == 0) {
-      constexpr uint32_t IDESC = idesc_bf16_f32(2 * BM, 256, false, kBackward);
+      constexpr uint32_t IDESC = idesc_bf16_f32(2 * BM, 256, false, kDz);
       int stage = 0, local = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -261,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk)
             umma_f16_ss_pair(d_tmem, smem_desc_sw128(a + kk * 32, 16, 1024),
-                             kBackward ? smem_desc_sw128(b + kk * 2048, 8192, 1024)
+                             kDz ? smem_desc_sw128(b + kk * 2048, 8192, 1024)
                                        : smem_desc_sw128(b + kk * 32, 16, 1024),
                              IDESC, (kb > 0 || kk > 0) ? 1u : 0u);
           umma_commit_pair(&empty[stage], 0x3);
@@ -292,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int m = row0 + lane;
       uint4 next_b[4], next_a[4];
       uint32_t next_e = 0;
-      if constexpr (kBackward) {  // the first chunk's saved tiles, in flight while the products finish
+      if constexpr (kDz) {  // the first chunk's saved tiles, in flight while the products finish
         const int n = n0 + chunk0 * 32;
         if (n < p.N && row0 < p.M) {
           gemm::warp_fetch_tile32(reinterpret_cast<const __nv_bfloat16*>(p.saved_b), p.ld_saved, row0, n, p.M, p.N, lane,
@@ -315,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = chunk0; c < chunk0 + kChunks; ++c) {
         const int n = n0 + c * 32;
         const bool live = n < p.N && row0 < p.M;  // warp-uniform
-        if constexpr (kBackward) {
+        if constexpr (kDz) {
           uint32_t r[32];
           tmem_ld_32x32b_x32(t_row + c * 32, r);
           uint4 cur_b[4], cur_a[4];
@@ -418,16 +405,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <int MODE>
-void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& o0, const CUtensorMap& o1,
-            const CUtensorMap& o2, const Params& p, int device, cudaStream_t stream) {
+cudaError_t launch_mode(const Maps& maps, const Params& p, int sms, int device, cudaStream_t stream) {
   auto kern = gated_kernel<MODE>;
   static bool configured[64] = {false};
   if (device < 0 || device >= 64 || !configured[device]) {
-    RX_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem)));
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
+    if (e != cudaSuccess) return e;
     if (device >= 0 && device < 64) configured[device] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * std::min(p.num_units, num_sms(device) / 2));
+  cfg.gridDim = dim3(2 * std::min(p.num_units, sms / 2));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
@@ -438,124 +425,16 @@ void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& o0,
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  RX_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, o0, o1, o2, p));
+  return cudaLaunchKernelEx(&cfg, kern, maps.a, maps.b, maps.out[0], maps.out[1], maps.out[2], p);
 }
 
-static void check_rows(const at::Tensor& t, const char* name, int64_t rows, int64_t cols, int device) {
-  RX_CHECK(t.is_cuda() && t.get_device() == device, name, " must be on the device of the first operand");
-  RX_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols && t.stride(1) == 1, name, " must be a row-major [",
-           rows, ", ", cols, "]");
-  RX_CHECK((t.stride(0) * t.element_size()) % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name,
-           " rows must be 16-byte aligned");
-}
-
-static void check_sizes(int64_t T, int64_t H, int64_t I) {
-  RX_CHECK(T > 0 && H > 0 && I > 0, "empty gated feed-forward");
-  RX_CHECK(H % 8 == 0 && I % 8 == 0, "hidden and intermediate sizes must be multiples of 8");
-  RX_CHECK(T < (1ll << 31) - 256 && H < (1ll << 30) && I < (1ll << 30), "gated feed-forward too large");
+cudaError_t launch(int mode, const Maps& maps, const Params& p, int sms, int device, cudaStream_t stream) {
+  switch (mode) {
+    case kForward: return launch_mode<kForward>(maps, p, sms, device, stream);
+    case kForwardSave: return launch_mode<kForwardSave>(maps, p, sms, device, stream);
+    default: return launch_mode<kBackward>(maps, p, sms, device, stream);
+  }
 }
 
 }  // namespace gated
-
-// h [T, I] = act(x Wg^T + bg) * (x Wu^T + bu) for x [T, H] and gate_up = [Wg; Wu] [2 I, H].
-// With `saved` (fp16 [T, 2 I]: b, then a) and `exps` (int16 [T, ceil(I / 32)]) it also keeps what
-// gated_backward reads.
-void gated_forward(const at::Tensor& x, const at::Tensor& gate_up, const c10::optional<at::Tensor>& bias,
-                   at::Tensor& h, const c10::optional<at::Tensor>& saved, const c10::optional<at::Tensor>& exps,
-                   int64_t act, const at::Tensor& status) {
-  check_bf16(x, "x");
-  check_bf16(gate_up, "gate_up");
-  check_bf16(h, "h");
-  RX_CHECK(x.dim() == 2 && gate_up.dim() == 2, "x and gate_up must be matrices");
-  const int64_t T = x.size(0), H = x.size(1), I = gate_up.size(0) / 2;
-  const int dev = x.get_device();
-  RX_CHECK(gate_up.size(0) == 2 * I, "gate_up must have an even number of rows");
-  gated::check_sizes(T, H, I);
-  gated::check_rows(x, "x", T, H, dev);
-  gated::check_rows(gate_up, "gate_up", 2 * I, H, dev);
-  gated::check_rows(h, "h", T, I, dev);
-  RX_CHECK(act >= 0 && act <= 3, "unknown activation code ", act);
-  RX_CHECK(saved.has_value() == exps.has_value(), "give saved and exps together");
-  gated::Params p{};
-  p.M = static_cast<int>(T);
-  p.N = static_cast<int>(I);
-  p.K = static_cast<int>(H);
-  p.m_tiles = static_cast<int>((T + 255) / 256);
-  p.n_tiles = static_cast<int>((I + 127) / 128);
-  RX_CHECK(static_cast<int64_t>(p.m_tiles) * p.n_tiles < (1ll << 31), "too many tiles");
-  p.num_units = p.m_tiles * p.n_tiles;
-  p.act = static_cast<int>(act);
-  p.status = status_ptr(status);
-  p.timeout_ns = kWaitBudgetNs;
-  if (bias.has_value()) {
-    check_bf16(*bias, "bias");
-    RX_CHECK(bias->get_device() == dev && bias->dim() == 1 && bias->numel() == 2 * I && bias->is_contiguous() &&
-                 reinterpret_cast<uintptr_t>(bias->data_ptr()) % 16 == 0,
-             "bias must be a contiguous 16-byte aligned [2 I] vector");
-    p.bias = reinterpret_cast<const __nv_bfloat16*>(bias->data_ptr());
-  }
-  c10::cuda::CUDAGuard guard(dev);
-  const CUtensorMap ta = make_tmap_2d_bf16(x.data_ptr(), T, H, x.stride(0), 64, gemm::BM);
-  const CUtensorMap tb = make_tmap_2d_bf16(gate_up.data_ptr(), 2 * I, H, gate_up.stride(0), 64, 128);
-  const CUtensorMap th = make_tmap_2d_bf16_store(h.data_ptr(), T, I, h.stride(0));
-  auto stream = at::cuda::getCurrentCUDAStream(dev).stream();
-  if (!saved.has_value()) {
-    gated::launch<0>(ta, tb, th, th, th, p, dev, stream);
-    return;
-  }
-  RX_CHECK(saved->scalar_type() == at::kHalf, "saved must be float16");
-  gated::check_rows(*saved, "saved", T, 2 * I, dev);
-  RX_CHECK(exps->is_cuda() && exps->get_device() == dev && exps->scalar_type() == at::kShort && exps->is_contiguous() &&
-               exps->dim() == 2 && exps->size(0) == T && exps->size(1) == (I + 31) / 32,
-           "exps must be a contiguous int16 [T, ceil(I / 32)]");
-  p.exps = reinterpret_cast<uint16_t*>(exps->data_ptr());
-  p.ld_exps = exps->size(1);
-  auto* sp = reinterpret_cast<__half*>(saved->data_ptr());
-  const CUtensorMap tb_out = make_tmap_2d_bf16_store(sp, T, I, saved->stride(0));
-  const CUtensorMap ta_out = make_tmap_2d_bf16_store(sp + I, T, I, saved->stride(0));
-  gated::launch<1>(ta, tb, th, tb_out, ta_out, p, dev, stream);
-}
-
-// dz [T, 2 I] = [dh b | dh a] with dh = dy Wd (dy [T, H], down [H, I]) and what gated_forward saved.
-void gated_backward(const at::Tensor& dy, const at::Tensor& down, const at::Tensor& saved, const at::Tensor& exps,
-                    at::Tensor& dz, const at::Tensor& status) {
-  check_bf16(dy, "dy");
-  check_bf16(down, "down");
-  check_bf16(dz, "dz");
-  RX_CHECK(dy.dim() == 2 && down.dim() == 2, "dy and down must be matrices");
-  const int64_t T = dy.size(0), H = dy.size(1), I = down.size(1);
-  const int dev = dy.get_device();
-  gated::check_sizes(T, H, I);
-  gated::check_rows(dy, "dy", T, H, dev);
-  gated::check_rows(down, "down", H, I, dev);
-  gated::check_rows(dz, "dz", T, 2 * I, dev);
-  RX_CHECK(saved.scalar_type() == at::kHalf, "saved must be float16");
-  gated::check_rows(saved, "saved", T, 2 * I, dev);
-  RX_CHECK(exps.is_cuda() && exps.get_device() == dev && exps.scalar_type() == at::kShort && exps.is_contiguous() &&
-               exps.dim() == 2 && exps.size(0) == T && exps.size(1) == (I + 31) / 32,
-           "exps must be a contiguous int16 [T, ceil(I / 32)]");
-  gated::Params p{};
-  p.M = static_cast<int>(T);
-  p.N = static_cast<int>(I);
-  p.K = static_cast<int>(H);
-  p.m_tiles = static_cast<int>((T + 255) / 256);
-  p.n_tiles = static_cast<int>((I + 255) / 256);
-  RX_CHECK(static_cast<int64_t>(p.m_tiles) * p.n_tiles < (1ll << 31), "too many tiles");
-  p.num_units = p.m_tiles * p.n_tiles;
-  p.status = status_ptr(status);
-  p.timeout_ns = kWaitBudgetNs;
-  p.saved_b = reinterpret_cast<const __half*>(saved.data_ptr());
-  p.saved_a = p.saved_b + I;
-  p.ld_saved = saved.stride(0);
-  p.exps = reinterpret_cast<uint16_t*>(exps.data_ptr());
-  p.ld_exps = exps.size(1);
-  c10::cuda::CUDAGuard guard(dev);
-  const CUtensorMap ta = make_tmap_2d_bf16(dy.data_ptr(), T, H, dy.stride(0), 64, gemm::BM);
-  const CUtensorMap tb = make_tmap_2d_bf16(down.data_ptr(), H, I, down.stride(0), 64, 64);
-  auto* zp = reinterpret_cast<__nv_bfloat16*>(dz.data_ptr());
-  const CUtensorMap t0 = make_tmap_2d_bf16_store(zp, T, I, dz.stride(0));
-  const CUtensorMap t1 = make_tmap_2d_bf16_store(zp + I, T, I, dz.stride(0));
-  gated::launch<2>(ta, tb, t0, t1, t1, p, dev, at::cuda::getCurrentCUDAStream(dev).stream());
-}
-
 }  // namespace rx

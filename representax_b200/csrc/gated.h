@@ -1,0 +1,38 @@
+// Host interface of the gated feed-forward kernels (gated.cu).
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace rx {
+namespace gated {
+
+// Forward; forward that keeps what the backward reads; backward (dz).
+enum Mode : int { kForward = 0, kForwardSave = 1, kBackward = 2 };
+
+struct Params {
+  int M, N, K;  // N: columns of h (forward) or of dh (backward)
+  int m_tiles, n_tiles, num_units;
+  int act;
+  const __nv_bfloat16* bias;  // forward: [2 N] (gate, up) or null
+  const __half* saved_b;      // backward: b [M, N], a [M, N] with row stride ld_saved
+  const __half* saved_a;
+  int64_t ld_saved;
+  uint16_t* exps;             // [M, ceil(N / 32)]: low byte the block exponent of b, high byte that of a
+  int64_t ld_exps;
+  int* status;
+  uint64_t timeout_ns;
+};
+
+// a: boxes of 128 rows x 64; b: 128 x 64 (forward, K-major) or 64 x 64 (backward, MN-major);
+// out: 32 x 32 store maps of h, b, a (forward) or of the two halves of dz.
+struct Maps {
+  CUtensorMap a, b, out[3];
+};
+
+cudaError_t launch(int mode, const Maps& maps, const Params& p, int sms, int device, cudaStream_t stream);
+
+}  // namespace gated
+}  // namespace rx

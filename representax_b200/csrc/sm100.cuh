@@ -338,6 +338,12 @@ __device__ __forceinline__ void red_add_f4(float4* addr, float4 v) {
                : "memory");
 }
 
+// Programmatic dependent launch: wait until the grids this one depends on have
+// completed (returns at once without such a launch) / let the dependent grid
+// start once every CTA has said so.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __device__ __forceinline__ int warp_id() { return threadIdx.x >> 5; }
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 31; }
 

@@ -30,9 +30,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import gemm as G
 from ._ext import ext, status
-from .ffn import rows16
 from .functional import _colsum_into, _GradSink, compute_view
 
 FORMATS = {"mxfp4": 1, "nvfp4": 2}
@@ -107,9 +105,8 @@ def quantize(x: torch.Tensor, fmt: str = "nvfp4", *, parts: int = 1) -> FP4Opera
         return _pack_reference(x, fmt, parts)
     if x.stride(1) != 1:
         x = x.contiguous()
-    op = empty_operand(x.shape[0], x.shape[1], fmt, x.device, parts)
-    ext().fp4_quantize(x, parts, FORMATS[fmt], op.data, op.scales, op.row_scale)
-    return op
+    data, scales, row = ext().fp4_quantize(x, parts, FORMATS[fmt])
+    return FP4Operand(data, scales, row, fmt, x.shape[1], parts)
 
 
 def dequantize(op: FP4Operand, dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -132,12 +129,6 @@ def _check_product(a_cols: int, b: FP4Operand, bias, residual, rows: int) -> Non
         raise ValueError(f"residual must be [{rows}, {b.rows}]")
 
 
-def _product(a: FP4Operand, b: FP4Operand, out, *, parts=1, act=0, bias=None, residual=None, q_out=None) -> None:
-    ext().fp4_gemm(a.data, a.scales, a.row_scale, b.data, b.scales, b.row_scale, a.k, FORMATS[a.fmt], parts, act, bias,
-                   residual, out, None if q_out is None else q_out.data, None if q_out is None else q_out.scales,
-                   status(a.device))
-
-
 def gemm(a: FP4Operand, b: FP4Operand, *, bias: torch.Tensor | None = None,
          residual: torch.Tensor | None = None) -> torch.Tensor:
     """``a b^T (+ bias) (+ residual)`` in bf16 for two operands of one format
@@ -154,53 +145,38 @@ def gemm(a: FP4Operand, b: FP4Operand, *, bias: torch.Tensor | None = None,
         y = _unpack_reference(a) @ _unpack_reference(b).T
         y = y if bias is None else y + bias.float()
         return (y if residual is None else y + residual.float()).to(torch.bfloat16)
-    out = torch.empty(a.rows, b.rows, dtype=torch.bfloat16, device=a.device)
-    if residual is not None and residual.stride(1) != 1:
-        residual = residual.contiguous()
-    if bias is not None:
-        bias = bias.contiguous()
-    n = b.rows // b.parts
-    for i in range(b.parts):
-        cut = slice(i * n, (i + 1) * n)
-        _product(a, b if b.parts == 1 else b.part(i), out if b.parts == 1 else out[:, cut],
-                 bias=None if bias is None else bias[cut], residual=None if residual is None else residual[:, cut])
-    return out
+    return ext().fp4_gemm(a.data, a.scales, a.row_scale, b.data, b.scales, b.row_scale, b.parts, a.k, FORMATS[a.fmt], bias,
+                          residual, status(a.device))
+
+
+def _linear(x, w: FP4Operand, bias, residual):
+    return ext().fp4_linear(x if x.stride(1) == 1 else x.contiguous(), w.data, w.scales, w.row_scale, w.parts,
+                            FORMATS[w.fmt], None if bias is None else compute_view(bias).contiguous(), residual,
+                            status(x.device))
 
 
 class LinearFP4Fn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, owner, bias, residual):
-        weight: FP4Operand = owner
-        y = gemm(quantize(x, weight.fmt), weight, bias=None if bias is None else compute_view(bias), residual=residual)
-        ctx.weight, ctx.has_b = weight, bias is not None
-        ctx.save_for_backward(bias if bias is not None else torch.empty(0, device=x.device))
-        return y
+    def forward(ctx, x, weight, bias, residual):
+        ctx.weight = weight
+        ctx.save_for_backward(bias)
+        return _linear(x, weight, bias, residual)
 
     @staticmethod
     def backward(ctx, dy):
         (bias,) = ctx.saved_tensors
         w = ctx.weight
-        dres = dy if ctx.needs_input_grad[3] else None
-        dx = None
-        sb = _GradSink(bias) if ctx.has_b else None
-        if dy.shape[0] == 0:
-            dx = dy.new_zeros(0, w.k) if ctx.needs_input_grad[0] else None
-            return dx, None, (torch.zeros_like(bias) if sb is not None and sb.wanted else None), dres
-        n, k = -(-w.rows // 8) * 8, -(-w.k // 8) * 8
-        if n != w.rows:  # the contraction dy W wants 16-byte rows of dy
-            padded = dy.new_zeros(dy.shape[0], n)
-            padded[:, :w.rows] = dy
-            dy = padded
-        dy = rows16(dy)
+        dx = db = None
         if ctx.needs_input_grad[0]:
-            wide = torch.empty(w.rows, k, dtype=torch.bfloat16, device=dy.device)
-            dequantize(w, out=wide[:, :w.k])
-            dx = torch.empty(dy.shape[0], k, dtype=torch.bfloat16, device=dy.device)
-            G.linear_dgrad(dy[:, :w.rows], wide[:, :w.k], out=dx[:, :w.k])
-            dx = dx[:, :w.k]
-        if sb is not None and sb.wanted:
-            _colsum_into(dy, sb) if n == w.rows else sb.buffer().add_(dy[:, :w.rows].float().sum(0))
-        return dx, None, (sb.result() if sb is not None else None), dres
+            dx = ext().fp4_linear_dgrad(dy, w.data, w.scales, w.row_scale, w.parts, w.k, FORMATS[w.fmt], status(dy.device))
+        if ctx.needs_input_grad[2]:
+            sink = _GradSink(bias)
+            if dy.shape[0] and dy.shape[1] % 8 == 0 and dy.is_contiguous() and dy.data_ptr() % 16 == 0:
+                _colsum_into(dy, sink)
+            else:
+                sink.buffer().add_(dy.float().sum(0))
+            db = sink.result()
+        return dx, None, db, dy if ctx.needs_input_grad[3] else None
 
 
 def linear_fp4(x: torch.Tensor, weight: FP4Operand, bias: torch.Tensor | None = None,
@@ -215,7 +191,9 @@ def linear_fp4(x: torch.Tensor, weight: FP4Operand, bias: torch.Tensor | None = 
     if x.is_cuda and x.dtype == torch.bfloat16:
         if residual is not None and residual.dtype != torch.bfloat16:
             raise TypeError("residual must be bfloat16 like x")
-        return LinearFP4Fn.apply(x, weight, bias, residual)
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, bias, residual)):
+            return LinearFP4Fn.apply(x, weight, bias, residual)
+        return _linear(x, weight, bias, residual)
     return linear_fp4_reference(x, weight, bias, residual)
 
 
@@ -247,17 +225,10 @@ def gated_feed_forward_fp4(x: torch.Tensor, gate_up: FP4Operand, down: FP4Operan
         return linear_fp4(h, down, down_bias, residual)
     if residual is not None and residual.dtype != torch.bfloat16:
         raise TypeError("residual must be bfloat16 like x")
-    b1 = None if gate_up_bias is None else compute_view(gate_up_bias).contiguous()
-    code = ACT_CODES[activation]
-    xq = quantize(x, gate_up.fmt)
-    if gate_up.fmt == "mxfp4" and down.fmt == "mxfp4":
-        hq = empty_operand(x.shape[0], down.k, "mxfp4", x.device)
-        _product(xq, gate_up, None, parts=2, act=code, bias=b1, q_out=hq)
-    else:
-        h = torch.empty(x.shape[0], down.k, dtype=torch.bfloat16, device=x.device)
-        _product(xq, gate_up, h, parts=2, act=code, bias=b1)
-        hq = quantize(h, down.fmt)
-    return gemm(hq, down, bias=None if down_bias is None else compute_view(down_bias), residual=residual)
+    bias = lambda t: None if t is None else compute_view(t).contiguous()  # noqa: E731
+    return ext().fp4_ffn(x if x.stride(1) == 1 else x.contiguous(), gate_up.data, gate_up.scales, gate_up.row_scale,
+                         FORMATS[gate_up.fmt], down.data, down.scales, down.row_scale, FORMATS[down.fmt],
+                         ACT_CODES[activation], bias(gate_up_bias), bias(down_bias), residual, status(x.device))
 
 
 # ------------------------------------------------------------ PyTorch statement
