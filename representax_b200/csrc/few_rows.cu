@@ -27,6 +27,7 @@
 
 #include <algorithm>
 
+#include "elect.cuh"
 #include "fp4.cuh"
 #include "gated_act.cuh"
 
@@ -153,31 +154,32 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      const uint32_t sf_cols = tmem_base + S::kAccCols;
-      bool issued_any = false;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const int i = kb - kb0, s = i % S::kStages;
-        if (*abort_flag || !mbar_wait(&full[s], (i / S::kStages) & 1, p.timeout_ns)) {
-          report_status(p.status, kStatusTimeoutMma);
-          *abort_flag = 1;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t w = smem_u32(base + s * S::kStage), x = w + PARTS * kTileW;
+    // (the whole warp runs the loop, one lane issues: operands stay in uniform registers)
+    const uint32_t sf_cols = tmem_base + S::kAccCols;
+    const uint64_t w0 = smem_desc_sw128(smem_u32(base), 16, 1024);
+    const uint64_t f0 = smem_desc_plain(smem_u32(base + S::kTiles), 512, 128);
+    bool ok = true, issued_any = false;
+    int s = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      ok = mbar_try_wait(&full[s], phase) || (*abort_flag == 0 && mbar_wait(&full[s], phase, p.timeout_ns));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t w = w0 + static_cast<uint32_t>(s * (S::kStage >> 4)), x = w + (PARTS * kTileW >> 4);
+      const uint32_t more = kb > kb0 ? 1u : 0u;
+      if (elect_one()) {
         if constexpr (KIND == kBf16) {
           constexpr uint32_t IDESC = idesc_bf16_f32(128, NT, false, false);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
             for (int b = 0; b < PARTS; ++b)
-              umma_f16_ss(tmem_base + b * NT, smem_desc_sw128(w + b * kTileW + kk * 32, 16, 1024),
-                          smem_desc_sw128(x + kk * 32, 16, 1024), IDESC, (i > 0 || kk > 0) ? 1u : 0u);
+              umma_f16_ss(tmem_base + b * NT, w + ((b * kTileW) >> 4) + kk * 2, x + kk * 2, IDESC, kk > 0 ? 1u : more);
         } else {
-          const uint32_t sf = w + S::kTiles;
+          const uint64_t f = f0 + static_cast<uint32_t>(s * (S::kStage >> 4));
 #pragma unroll
-          for (int a = 0; a < (PARTS + 1) * S::kGroups; ++a)
-            tmem_cp_32x128b_warpx4(sf_cols + 4 * a, smem_desc_plain(sf + a * 512, 512, 128));
+          for (int a = 0; a < (PARTS + 1) * S::kGroups; ++a) tmem_cp_32x128b_warpx4(sf_cols + 4 * a, f + 32 * a);
           // 64-value steps past K would multiply zeros by scales that nothing defines
           const int steps = min(4, (p.K - kb * fp4::kStageK + 63) / 64);
 #pragma unroll
@@ -187,20 +189,28 @@ __global__ void __launch_bounds__(kThreads, 2)
               const uint32_t id = KIND == kMxfp4 ? 2u * (kk & 1) : 0u;
 #pragma unroll
               for (int b = 0; b < PARTS; ++b)
-                fp4::umma<KIND>(tmem_base + b * NT, smem_desc_sw128(w + b * kTileW + kk * 32, 16, 1024),
-                                smem_desc_sw128(x + kk * 32, 16, 1024), fp4::idesc(128, NT, KIND, id),
-                                (sf_cols + 4 * (b * S::kGroups + atom)) | (id << 30),
-                                (sf_cols + 4 * (PARTS * S::kGroups + atom)) | (id << 30), (i > 0 || kk > 0) ? 1u : 0u);
+                fp4::umma<KIND>(tmem_base + b * NT, w + ((b * kTileW) >> 4) + kk * 2, x + kk * 2,
+                                fp4::idesc(128, NT, KIND, id), (sf_cols + 4 * (b * S::kGroups + atom)) | (id << 30),
+                                (sf_cols + 4 * (PARTS * S::kGroups + atom)) | (id << 30), kk > 0 ? 1u : more);
             }
           }
         }
-        issued_any = true;
         umma_commit(&empty[s]);
       }
-      // one arrival even without work (fewer K blocks than CTAs cannot happen, an abort can)
-      umma_commit(done);
-      if (issued_any && !mbar_wait(done, 0, p.timeout_ns)) report_status(p.status, kStatusTimeoutDrain);
+      __syncwarp();
+      issued_any = true;
+      if (++s == S::kStages) {
+        s = 0;
+        phase ^= 1;
+      }
     }
+    if (!ok) {
+      if (lane == 0) report_status(p.status, kStatusTimeoutMma);
+      *abort_flag = 1;
+    }
+    if (elect_one()) umma_commit(done);
+    if (lane == 0 && issued_any && !mbar_wait(done, 0, p.timeout_ns)) report_status(p.status, kStatusTimeoutDrain);
+    __syncwarp();
   }
   __syncthreads();  // every MMA has completed and no copy is in flight: the ring may be reused
   float* part = reinterpret_cast<float*>(base);
@@ -266,10 +276,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         y[j] = v[0][j];
-        if constexpr (PARTS == 2) y[j] = gated::act_value(v[0][j], p.act) * v[1][j];
+        if constexpr (PARTS == 2) y[j] = v[1][j];
         if constexpr (PARTS == 1)
           if (n + j < p.N && p.residual != nullptr) y[j] += __bfloat162float(p.residual[t * p.ld_res + n + j]);
       }
+      if constexpr (PARTS == 2) gated::gate(p.act, v[0], y);
       if constexpr (PARTS == 2 && KIND == kMxfp4) {
         if (p.q_out != nullptr) {  // eight lanes hold a block of 32
           uint32_t top = 0;

@@ -177,6 +177,22 @@ void run_dequantize(const Operand& o, at::Tensor& out, cudaStream_t stream) {
   check_launch(fp4::dequantize(p, o.fmt, type, stream), "fp4_dequantize");
 }
 
+// Tensor map of an operand's scales: rows of 512 bytes (128 32-bit words), boxes of one stage's groups.
+CUtensorMap scale_map(const Operand& o) {
+  CUtensorMap map;
+  const int64_t rows = o.scale_bytes() / 512;
+  RX_CHECK(rows < (1ll << 31), "too many scale groups");
+  cuuint64_t dims[2] = {128u, static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {512u};
+  cuuint32_t box[2] = {128u, o.fmt == kMx ? 2u : 4u};
+  cuuint32_t elem_strides[2] = {1, 1};
+  const CUresult r = encode_tiled_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, o.sf, dims, strides, box, elem_strides,
+                                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  RX_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (scales) failed with code ", static_cast<int>(r));
+  return map;
+}
+
 // out = a b^T (+ bias) (+ residual) for one part of b; act(a bg^T + bg) * (a bu^T + bu) for two, into
 // `out` or, in MXFP4, into the operand `q_out`. `after_producer`: a was written by the launch just before, which
 // lets this one start early.
@@ -191,9 +207,6 @@ void run_product(const Operand& a, const Operand& b, int64_t act, const OptTenso
   if (out != nullptr) check_matrix(*out, "out", M, N, dev);
   if (residual.has_value()) check_matrix(*residual, "residual", M, N, dev);
   if (M == 0 || N == 0) return;
-  const bool few = M <= few::kMaxRows;
-  const CUtensorMap ta = make_tmap_2d_u8(a.q, M, a.code_bytes(), a.ldq, few ? few::tile_rows(M) : 128);
-  const CUtensorMap tb = make_tmap_2d_u8(b.q, b.all_rows(), b.code_bytes(), b.ldq, 128);
   auto* out_p = out != nullptr ? reinterpret_cast<__nv_bfloat16*>(out->data_ptr()) : nullptr;
   const auto* res_p = residual.has_value() ? reinterpret_cast<const __nv_bfloat16*>(residual->data_ptr()) : nullptr;
   auto fill = [&](auto& p) {
@@ -216,7 +229,9 @@ void run_product(const Operand& a, const Operand& b, int64_t act, const OptTenso
     p.status = status_ptr(status);
     p.timeout_ns = kWaitBudgetNs;
   };
-  if (few) {
+  const CUtensorMap tb = make_tmap_2d_u8(b.q, b.all_rows(), b.code_bytes(), b.ldq, 128);
+  if (M <= few::kMaxRows) {
+    const CUtensorMap ta = make_tmap_2d_u8(a.q, M, a.code_bytes(), a.ldq, few::tile_rows(M));
     few::Params p{};
     fill(p);
     p.T = static_cast<int>(M);
@@ -233,17 +248,25 @@ void run_product(const Operand& a, const Operand& b, int64_t act, const OptTenso
   fp4::GemmParams p{};
   fill(p);
   p.M = static_cast<int>(M);
-  p.m_tiles = static_cast<int>(row_tiles(M));
+  p.m_tiles = static_cast<int>((M + 255) / 256);
   p.n_tiles = static_cast<int>(b.parts == 2 ? (N + 127) / 128 : (N + 255) / 256);
   RX_CHECK(static_cast<int64_t>(p.m_tiles) * p.n_tiles < (1ll << 31), "too many tiles");
   p.k_stages = static_cast<int>((K + 255) / 256);
-  p.sf_a = a.sf;
-  p.sf_b = b.sf;
+  p.a_tiles = static_cast<int>(row_tiles(M));
+  p.b_tiles = static_cast<int>(row_tiles(N));
   p.row_a = a.row;
   p.row_b = b.row;
   p.vec = (out == nullptr || aligned_rows(*out)) && (!residual.has_value() || aligned_rows(*residual)) &&
           (!bias.has_value() || (aligned_rows(*bias) && (b.parts == 1 || N % 8 == 0)));
-  check_launch(fp4::gemm(ta, tb, p, a.fmt, num_sms(dev), dev, stream), "fp4 product");
+  p.vec_rows = b.row != nullptr && reinterpret_cast<uintptr_t>(b.row) % 16 == 0 && (b.parts == 1 || N % 4 == 0);
+  fp4::GemmMaps maps;
+  maps.a = make_tmap_2d_u8(a.q, M, a.code_bytes(), a.ldq, 128);
+  maps.b = tb;
+  maps.sf_a = scale_map(a);
+  maps.sf_b = scale_map(b);
+  maps.out = maps.a;
+  if (p.vec && out != nullptr) maps.out = make_tmap_2d_bf16_store(out_p, M, N, p.ld_out);
+  check_launch(fp4::gemm(maps, p, a.fmt, num_sms(dev), dev, stream), "fp4 product");
 }
 
 // out [M, parts * N] = a b^T (+ bias) (+ residual), part by part.

@@ -41,11 +41,10 @@ cudaError_t dequantize(const DequantParams& p, int fmt, int type, cudaStream_t s
 
 struct GemmParams {
   int M, N, K;         // N: output columns (per part)
-  int m_tiles, n_tiles, k_stages;
+  int m_tiles, n_tiles, k_stages;  // tiles of 256 rows x 256 columns (gated: 128)
   int gated, act;      // gated: B parts [gate; up], output act(g) * u
-  const uint8_t* sf_a;
-  const uint8_t* sf_b;
   int64_t groups;      // K groups of both scale arrays
+  int a_tiles, b_tiles;  // scale row tiles of A and of one part of B
   const float* row_a;  // NVFP4 row factors [M], [parts * N]
   const float* row_b;
   const __nv_bfloat16* bias;      // [parts * N] or null
@@ -53,7 +52,8 @@ struct GemmParams {
   int64_t ld_res;
   __nv_bfloat16* out;  // [M, N], or null with q_out
   int64_t ld_out;
-  int vec;             // out / residual / bias rows allow 16-byte accesses
+  int vec;             // rows of out, residual and bias are 16-byte aligned: `map_out` is valid
+  int vec_rows;        // row_b allows 16-byte loads at multiples of four columns
   uint8_t* q_out;      // gated MXFP4 output: codes [M, ld_q] and scales
   int64_t ld_q;
   uint8_t* q_sf;
@@ -62,9 +62,13 @@ struct GemmParams {
   uint64_t timeout_ns;
 };
 
-// Boxes of 128 rows x 128 bytes for both maps.
-cudaError_t gemm(const CUtensorMap& map_a, const CUtensorMap& map_b, const GemmParams& p, int fmt, int sms, int device,
-                 cudaStream_t stream);
+// a, b: codes, boxes of 128 rows x 128 bytes. sf_a, sf_b: scales as 512-byte rows of 32-bit words, boxes of
+// one stage's groups. out: 32 x 32 store map.
+struct GemmMaps {
+  CUtensorMap a, b, sf_a, sf_b, out;
+};
+
+cudaError_t gemm(const GemmMaps& maps, const GemmParams& p, int fmt, int sms, int device, cudaStream_t stream);
 
 }  // namespace fp4
 }  // namespace rx

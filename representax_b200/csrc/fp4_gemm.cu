@@ -10,36 +10,40 @@
 // one scale block, so the fp32 product is quantised without a trip through
 // memory or through bf16.
 //
-// Persistent, one CTA per SM: producer warp (TMA of a 128 x 256 A tile and two
-// 128 x 256 B tiles per stage, 48 KB, and the stage's scales by bulk copies), one
-// issuing thread (scales to TMEM, then four K = 64 MMAs of 128 x 256), eight
-// epilogue warps. The two B tiles are adjacent columns, or the gate and up
-// rows of the same 128 columns. The accumulator takes 256 of the 512 TMEM
-// columns and the scales of all stages share the rest; instead of a second
+// Persistent CTA pairs on tiles of 256 x 256 accumulators. CTA r of a pair loads
+// A rows [128 r, 128 r + 128) and half of the B rows (plain: adjacent columns;
+// gated: CTA 0 the gate rows, CTA 1 the up rows of the same 128 columns), 32 KB of
+// codes per 256 values of K, with the scales of its A rows and of all B rows. One
+// thread copies the scales to TMEM (one stage ahead of the products, so that the
+// copies do not stand between them) and issues four K = 64 MMAs of 256 x 256 per
+// stage; eight epilogue warps per CTA. The accumulator takes 256 of the 512 TMEM
+// columns, the scales of all stages share the rest; instead of a second
 // accumulator, an epilogue thread takes its 128 values into registers and
-// frees the accumulator before it computes or stores, so the tensor core waits for a
-// TMEM read only.
+// frees the accumulator before it computes or stores, so the tensor core waits
+// for a TMEM read only. bf16 results leave through shared memory and TMA tile stores.
 #include "fp4.h"
 
 #include <algorithm>
 
 #include "fp4.cuh"
 #include "gated_act.cuh"
+#include "tile_io.cuh"
 
 namespace rx {
 namespace fp4 {
 
 constexpr int kTile = 128 * 128;   // 128 rows x 256 codes
-constexpr int kTiles = 3 * kTile;
-constexpr int kGemmStages = 4;
+constexpr int kGemmStages = 5;
 constexpr int kEpiWarps = 8;
 constexpr int kGemmThreads = 32 * (2 + kEpiWarps);
+constexpr int kStaging = kEpiWarps * 2 * 2048;
 
 template <int FMT>
 struct GemmShape {
   static constexpr int kGroups = groups_per_stage(FMT);
-  static constexpr int kSf = 3 * kGroups * 512;
-  static constexpr size_t kSmem = 1024 + kGemmStages * (kTiles + kSf) + 256;
+  static constexpr int kSf = 3 * kGroups * 512;    // one A tile's scales, two B tiles'
+  static constexpr int kStage = 2 * kTile + kSf;
+  static constexpr size_t kSmem = 1024 + kGemmStages * kStage + kStaging + 256;
   static constexpr int kSfCols = 3 * kGroups * 4;  // TMEM columns of a stage's scales
   static_assert(256 + kGemmStages * kSfCols <= 512 && kSmem <= 232448, "does not fit");
 };
@@ -92,19 +96,35 @@ __device__ __forceinline__ void finish32(const GemmParams& p, float row_a, int64
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
   if constexpr (FMT == kNv) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (n + i < p.N) v[i] *= row_a * p.row_b[part0 + n + i];
+    for (int q = 0; q < 8; ++q) {
+      float4 f;
+      if (p.vec_rows && n + 32 <= p.N) {
+        f = *reinterpret_cast<const float4*>(p.row_b + part0 + n + 4 * q);
+      } else {
+        f.x = n + 4 * q < p.N ? p.row_b[part0 + n + 4 * q] : 0.f;
+        f.y = n + 4 * q + 1 < p.N ? p.row_b[part0 + n + 4 * q + 1] : 0.f;
+        f.z = n + 4 * q + 2 < p.N ? p.row_b[part0 + n + 4 * q + 2] : 0.f;
+        f.w = n + 4 * q + 3 < p.N ? p.row_b[part0 + n + 4 * q + 3] : 0.f;
+      }
+      v[4 * q] *= row_a * f.x;
+      v[4 * q + 1] *= row_a * f.y;
+      v[4 * q + 2] *= row_a * f.z;
+      v[4 * q + 3] *= row_a * f.w;
+    }
   }
   if (p.bias != nullptr) add32(p.bias + part0 + n, p.vec, n, p.N, v);
 }
 
 template <int FMT, bool GATED>
 __global__ void __launch_bounds__(kGemmThreads, 1)
-    fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmParams p) {
+    fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmSfA, const __grid_constant__ CUtensorMap tmSfB,
+                    const __grid_constant__ CUtensorMap tmOut, const GemmParams p) {
   using S = GemmShape<FMT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sf_base = base + kGemmStages * kTiles;
+  uint8_t* sC = base + kGemmStages * 2 * kTile;  // code tiles, then staging, then scales
+  uint8_t* sf_base = sC + kStaging;
   uint64_t* full = reinterpret_cast<uint64_t*>(sf_base + kGemmStages * S::kSf);
   uint64_t* empty = full + kGemmStages;
   uint64_t* tfull = empty + kGemmStages;
@@ -113,6 +133,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = warp_id(), lane = lane_id();
+  const int rank = static_cast<int>(cluster_ctarank());
+  const bool leader = rank == 0;
+  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
   constexpr int kTileN = GATED ? 128 : 256;  // output columns of a tile
 
   if (threadIdx.x == 0) {
@@ -121,35 +144,40 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       mbar_init(&empty[s], 1);
     }
     mbar_init(tfull, 1);
-    mbar_init(tempty, kEpiWarps);
+    mbar_init(tempty, 2 * kEpiWarps);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbarrier_init();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
   }
   tc_fence_before();
-  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers are initialised before any remote use
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int num_units = p.m_tiles * p.n_tiles;
-  const int b_tiles = (p.N + 127) >> 7;  // scale row tiles of one part of B
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       tma_prefetch_map(&tmA);
       tma_prefetch_map(&tmB);
+      tma_prefetch_map(&tmSfA);
+      tma_prefetch_map(&tmSfB);
+      const uint32_t full_leader0 = mapa_shared(smem_u32(&full[0]), 0);
+      const int groups = static_cast<int>(p.groups);
       int stage = 0;
-      uint32_t phase = 0, issued = 0, parity = 0;
+      uint32_t phase = 0;
       bool ok = true;
-      for (int u = blockIdx.x; ok && u < num_units; u += gridDim.x) {
+      for (int u = cluster; ok && u < num_units; u += clusters) {
         const int mt = u % p.m_tiles, nt = u / p.m_tiles;
-        // rows and scale tiles of the two B tiles (a second tile past the end reads the last one's scales)
-        const int row0 = nt * kTileN, row1 = GATED ? row0 + p.N : row0 + 128;
-        const int64_t t0 = row0 >> 7, t1 = GATED ? t0 + b_tiles : min(static_cast<int>(t0) + 1, b_tiles - 1);
+        const int m_row = mt * 256 + rank * 128;
+        const int b_row = GATED ? nt * 128 + rank * p.N : nt * 256 + rank * 128;
+        // scale row tiles (a tile past the end reads the last one's: its products are dropped)
+        const int ta = min(2 * mt + rank, p.a_tiles - 1);
+        const int tb0 = GATED ? nt : 2 * nt, tb1 = GATED ? nt + p.b_tiles : min(2 * nt + 1, p.b_tiles - 1);
         for (int ks = 0; ks < p.k_stages; ++ks) {
           if (*abort_flag || !mbar_wait(&empty[stage], phase ^ 1, p.timeout_ns)) {
             report_status(p.status, kStatusTimeoutProducer);
@@ -157,93 +185,124 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&full[stage], kTiles + S::kSf);
-          uint8_t* tiles = base + stage * kTiles;
+          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * S::kStage);  // both CTAs' loads
+          const uint32_t bar = full_leader0 + stage * 8;
+          uint8_t* tiles = base + stage * 2 * kTile;
           uint8_t* sf = sf_base + stage * S::kSf;
           constexpr int kBytes = S::kGroups * 512;
-          const int64_t g = static_cast<int64_t>(ks) * S::kGroups;
-          tma_load_2d(tiles, &tmA, &full[stage], ks * 128, mt * 128);
-          tma_load_2d(tiles + kTile, &tmB, &full[stage], ks * 128, row0);
-          tma_load_2d(tiles + 2 * kTile, &tmB, &full[stage], ks * 128, row1);
-          bulk_load(sf, p.sf_a + (mt * p.groups + g) * 512, kBytes, &full[stage]);
-          bulk_load(sf + kBytes, p.sf_b + (t0 * p.groups + g) * 512, kBytes, &full[stage]);
-          bulk_load(sf + 2 * kBytes, p.sf_b + (t1 * p.groups + g) * 512, kBytes, &full[stage]);
-          issued |= 1u << stage;
-          parity = (parity & ~(1u << stage)) | (phase << stage);
+          const int g = ks * S::kGroups;
+          tma_load_2d_pair(tiles, &tmA, bar, ks * 128, m_row);
+          tma_load_2d_pair(tiles + kTile, &tmB, bar, ks * 128, b_row);
+          tma_load_2d_pair(sf, &tmSfA, bar, 0, ta * groups + g);
+          tma_load_2d_pair(sf + kBytes, &tmSfB, bar, 0, tb0 * groups + g);
+          tma_load_2d_pair(sf + 2 * kBytes, &tmSfB, bar, 0, tb1 * groups + g);
           if (++stage == kGemmStages) {
             stage = 0;
             phase ^= 1;
           }
         }
       }
-      // leave no copy in flight into shared memory that is about to be released
-      for (int s = 0; s < kGemmStages; ++s)
-        if (((issued >> s) & 1u) && !mbar_wait(&full[s], (parity >> s) & 1u, p.timeout_ns))
+      // every load was consumed once the MMAs of its stage have committed
+      for (int s = 0; s < kGemmStages; ++s) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, p.timeout_ns)) {
           report_status(p.status, kStatusTimeoutDrain);
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      int stage = 0, local = 0;
-      uint32_t phase = 0;
-      bool ok = true, issued_any = false;
-      for (int u = blockIdx.x; ok && u < num_units; u += gridDim.x, ++local) {
-        if (*abort_flag || !mbar_wait(tempty, (local & 1) ^ 1, p.timeout_ns)) {
-          report_status(p.status, kStatusTimeoutMma);
-          *abort_flag = 1;
           break;
         }
-        tc_fence_after();
-        for (int ks = 0; ks < p.k_stages; ++ks) {
-          if (*abort_flag || !mbar_wait(&full[stage], phase, p.timeout_ns)) {
-            report_status(p.status, kStatusTimeoutMma);
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t a = smem_u32(base + stage * kTiles), b = a + kTile;
-          const uint32_t sf = smem_u32(sf_base + stage * S::kSf);
-          const uint32_t sfa = tmem_base + 256 + stage * S::kSfCols, sfb = sfa + 4 * S::kGroups;
-#pragma unroll
-          for (int j = 0; j < S::kGroups; ++j) {
-            tmem_cp_32x128b_warpx4(sfa + 4 * j, smem_desc_plain(sf + j * 512, 512, 128));
-            tmem_cp_32x128b_warpx4(sfb + 8 * j, smem_desc_plain(sf + (S::kGroups + j) * 512, 512, 128));
-            tmem_cp_32x128b_warpx4(sfb + 8 * j + 4, smem_desc_plain(sf + (2 * S::kGroups + j) * 512, 512, 128));
-          }
-          // 64-value steps past K would multiply zeros by scales that nothing defines
-          const int steps = min(4, (p.K - ks * kStageK + 63) / 64);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            if (kk < steps) {
-              const int atom = FMT == kMx ? kk >> 1 : kk;
-              const uint32_t id = FMT == kMx ? 2u * (kk & 1) : 0u;
-              umma<FMT>(tmem_base, smem_desc_sw128(a + kk * 32, 16, 1024), smem_desc_sw128(b + kk * 32, 16, 1024),
-                        idesc(128, 256, FMT, id), (sfa + 4 * atom) | (id << 30), (sfb + 8 * atom) | (id << 30),
-                        (ks > 0 || kk > 0) ? 1u : 0u);
-            }
-          }
-          issued_any = true;
-          umma_commit(&empty[stage]);
-          if (++stage == kGemmStages) {
-            stage = 0;
-            phase ^= 1;
-          }
+        if (++stage == kGemmStages) {
+          stage = 0;
+          phase ^= 1;
         }
-        if (!ok) break;
-        umma_commit(tfull);
-      }
-      if (issued_any) {
-        umma_commit(drain);
-        if (!mbar_wait(drain, 0, p.timeout_ns)) report_status(p.status, kStatusTimeoutDrain);
       }
     }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (even CTA)
+    if (leader) {
+      // The whole warp runs this loop and one lane issues. What the issuing costs bounds the stage, so its
+      // instructions are kept few: descriptors are a base plus an offset in their address field, and the abort
+      // flag is read only where a wait is not over at once.
+      const uint64_t a0 = smem_desc_sw128(smem_u32(base), 16, 1024);
+      const uint64_t f0 = smem_desc_plain(smem_u32(sf_base), 512, 128);
+      const uint32_t tmem_sf = tmem_base + 256;
+      auto ready = [&](uint64_t* bar, uint32_t parity) -> bool {
+        const bool now = mbar_try_wait(bar, parity) || (*abort_flag == 0 && mbar_wait(bar, parity, p.timeout_ns));
+        return __all_sync(0xffffffffu, now);
+      };
+      // Wait for a stage's data and copy its scales into the stage's TMEM columns.
+      auto fetch = [&](int s, uint32_t phase) -> bool {
+        if (!ready(&full[s], phase)) return false;
+        tc_fence_after();
+        const uint64_t f = f0 + static_cast<uint32_t>(s * (S::kSf >> 4));
+        const uint32_t sfa = tmem_sf + s * S::kSfCols, sfb = sfa + 4 * S::kGroups;
+        if (elect_one()) {
+#pragma unroll
+          for (int j = 0; j < S::kGroups; ++j) {
+            tmem_cp_scales_pair(sfa + 4 * j, f + 32 * j);
+            tmem_cp_scales_pair(sfb + 8 * j, f + 32 * (S::kGroups + j));
+            tmem_cp_scales_pair(sfb + 8 * j + 4, f + 32 * (2 * S::kGroups + j));
+          }
+        }
+        return true;
+      };
+      auto products = [&](int s, int kk, uint32_t accumulate) {
+        const uint64_t a = a0 + static_cast<uint32_t>(s * (2 * kTile >> 4) + kk * 2);
+        const uint32_t sfa = tmem_sf + s * S::kSfCols, sfb = sfa + 4 * S::kGroups;
+        const int atom = FMT == kMx ? kk >> 1 : kk;
+        const uint32_t id = FMT == kMx ? 2u * (kk & 1) : 0u;
+        umma_pair<FMT>(tmem_base, a, a + (kTile >> 4), idesc(256, 256, FMT, id), (sfa + 4 * atom) | (id << 30),
+                       (sfb + 8 * atom) | (id << 30), accumulate);
+      };
+      const int tail = (p.K - (p.k_stages - 1) * kStageK + 63) / 64;  // 64-value steps of the last stage
+      int s = 0, local = 0;
+      uint32_t phase = 0;
+      bool ok = cluster >= num_units || fetch(0, 0);
+      for (int u = cluster; ok && u < num_units; u += clusters, ++local) {
+        ok = ready(tempty, static_cast<uint32_t>(local & 1) ^ 1u);
+        tc_fence_after();
+        for (int ks = 0; ok && ks < p.k_stages; ++ks) {
+          int s1 = s + 1;
+          if (s1 == kGemmStages) {
+            s1 = 0;
+            phase ^= 1;
+          }
+          const bool last = ks + 1 == p.k_stages;
+          if (!last || u + clusters < num_units) ok = fetch(s1, phase);  // one stage ahead
+          if (!ok) break;
+          if (elect_one()) {
+            if (!last || tail == 4) {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk) products(s, kk, (ks > 0 || kk > 0) ? 1u : 0u);
+            } else {  // steps past K would multiply zeros by scales that nothing defines
+              for (int kk = 0; kk < tail; ++kk) products(s, kk, (ks > 0 || kk > 0) ? 1u : 0u);
+            }
+            umma_commit_pair(&empty[s], 0x3);
+            if (last) umma_commit_pair(tfull, 0x3);
+          }
+          __syncwarp();
+          s = s1;
+        }
+      }
+      if (!ok) {
+        if (lane == 0) report_status(p.status, kStatusTimeoutMma);
+        *abort_flag = 1;
+      }
+      if (elect_one()) umma_commit_pair(drain, 0x3);
+    }
+    if (lane == 0 && !mbar_wait(drain, 0, p.timeout_ns)) report_status(p.status, kStatusTimeoutDrain);
+    __syncwarp();
   } else {
-    // ------------------------------------------------------------ epilogue
+    // ------------------------------------------------------------ epilogue (both CTAs)
     const int quad = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t tempty_leader = mapa_shared(smem_u32(tempty), 0);
+    uint8_t* const staging = sC + (warp - 2) * 4096;
     int local = 0;
-    for (int u = blockIdx.x; u < num_units; u += gridDim.x, ++local) {
+    uint32_t seq = 0;
+    for (int u = cluster; u < num_units; u += clusters, ++local) {
       const int mt = u % p.m_tiles, nt = u / p.m_tiles;
+      const int row0 = mt * 256 + rank * 128 + quad * 32;  // this warp's 32 rows
+      uint4 next[4];  // the next chunk's residual tile, in flight
+      const bool side = !GATED && p.residual != nullptr && p.vec && row0 < p.M;
+      if (side && nt * kTileN + half * 128 < p.N)
+        gemm::warp_fetch_tile32(p.residual, p.ld_res, row0, nt * kTileN + half * 128, p.M, p.N, lane, next);
       bool ok = (*abort_flag == 0) && mbar_wait(tfull, local & 1, p.timeout_ns);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
@@ -261,10 +320,37 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(tempty);
-      const int64_t m = static_cast<int64_t>(mt) * 128 + quad * 32 + lane;
-      if (m >= p.M) continue;
-      const float row_a = FMT == kNv ? p.row_a[m] : 1.f;
+      if (lane == 0) mbar_arrive_cluster(tempty_leader);
+      if (row0 >= p.M) continue;  // warp-uniform
+      const int64_t m = row0 + lane;
+      const bool live = m < p.M;
+      const float row_a = FMT == kNv && live ? p.row_a[m] : 1.f;
+      // 32 outputs of every row of the warp, from column n
+      auto put = [&](int n, float (&v)[32], const uint4* res) {
+        if (!p.vec) {
+          if (live) store32(p, m, n, v);
+          return;
+        }
+        uint8_t* buf = staging + (seq++ & 1) * 2048;
+        if (lane == 0) tma_store_wait_read<1>();  // the store that last read `buf` is done reading
+        __syncwarp();
+        if (res != nullptr) {  // the tile's rows to their threads
+          float add[32];
+          gemm::warp_put_tile32_sw64(buf, lane, *reinterpret_cast<const uint4(*)[4]>(res));
+          __syncwarp();
+          gemm::read_row32_sw64(buf, lane, add);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += add[i];
+        }
+        gemm::stage_row32_sw64(buf, lane, v);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&tmOut, buf, n, row0);
+          tma_store_commit();
+        }
+      };
       if constexpr (GATED) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -274,9 +360,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           float g[32], v[32];
           finish32<FMT>(p, row_a, 0, n, r[c], g);
           finish32<FMT>(p, row_a, p.N, n, r[2 + c], v);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = n + i < p.N ? v[i] * gated::act_value(g[i], p.act) : 0.f;
+          gated::gate(p.act, g, v);
           if (FMT == kMx && p.q_out != nullptr) {
+            if (!live) continue;
+            if (n + 32 > p.N) {  // columns past the end: zeros in the next layer's contraction
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (n + i >= p.N) v[i] = 0.f;
+            }
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
@@ -294,7 +385,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
               *reinterpret_cast<uint4*>(p.q_out + m * p.ld_q + (n >> 1)) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
             p.q_sf[scale_offset(m, n >> 5, p.q_groups)] = static_cast<uint8_t>(byte);
           } else {
-            store32(p, m, n, v);
+            put(n, v, nullptr);
           }
         }
       } else {
@@ -304,22 +395,33 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           if (n >= p.N) continue;
           float v[32];
           finish32<FMT>(p, row_a, 0, n, r[c], v);
-          if (p.residual != nullptr) add32(p.residual + m * p.ld_res + n, p.vec, n, p.N, v);
-          store32(p, m, n, v);
+          if (side) {
+            uint4 cur[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) cur[q] = next[q];
+            if (c < 3 && n + 32 < p.N)
+              gemm::warp_fetch_tile32(p.residual, p.ld_res, row0, n + 32, p.M, p.N, lane, next);
+            put(n, v, cur);
+          } else {
+            if (p.residual != nullptr && live) add32(p.residual + m * p.ld_res + n, false, n, p.N, v);
+            put(n, v, nullptr);
+          }
         }
       }
     }
+    if (lane == 0) tma_store_wait<0>();  // every tile store has landed before the CTA exits
+    __syncwarp();
   }
 
   tc_fence_before();
   __syncthreads();
+  cluster_sync_all();  // no CTA leaves while its peer may still signal it
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem_base, 512);
+  if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
 }
 
 template <int FMT, bool GATED>
-cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams& p, int sms, int device,
-                   cudaStream_t stream) {
+cudaError_t launch(const GemmMaps& maps, const GemmParams& p, int sms, int device, cudaStream_t stream) {
   auto kern = fp4_gemm_kernel<FMT, GATED>;
   constexpr size_t smem = GemmShape<FMT>::kSmem;
   static bool configured[64] = {false};
@@ -328,17 +430,25 @@ cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParam
     if (e != cudaSuccess) return e;
     if (device >= 0 && device < 64) configured[device] = true;
   }
-  kern<<<std::min(p.m_tiles * p.n_tiles, sms), kGemmThreads, smem, stream>>>(ta, tb, p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * std::min(p.m_tiles * p.n_tiles, sms / 2));
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, maps.a, maps.b, maps.sf_a, maps.sf_b, maps.out, p);
 }
 
-cudaError_t gemm(const CUtensorMap& map_a, const CUtensorMap& map_b, const GemmParams& p, int fmt, int sms, int device,
-                 cudaStream_t stream) {
+cudaError_t gemm(const GemmMaps& maps, const GemmParams& p, int fmt, int sms, int device, cudaStream_t stream) {
   if (fmt == kMx)
-    return p.gated ? launch<kMx, true>(map_a, map_b, p, sms, device, stream)
-                   : launch<kMx, false>(map_a, map_b, p, sms, device, stream);
-  return p.gated ? launch<kNv, true>(map_a, map_b, p, sms, device, stream)
-                 : launch<kNv, false>(map_a, map_b, p, sms, device, stream);
+    return p.gated ? launch<kMx, true>(maps, p, sms, device, stream) : launch<kMx, false>(maps, p, sms, device, stream);
+  return p.gated ? launch<kNv, true>(maps, p, sms, device, stream) : launch<kNv, false>(maps, p, sms, device, stream);
 }
 
 }  // namespace fp4

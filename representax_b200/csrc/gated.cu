@@ -36,6 +36,7 @@
 #include <algorithm>
 
 #include "gated_act.cuh"
+#include "elect.cuh"
 #include "sm100.cuh"
 #include "tile_io.cuh"
 
@@ -222,45 +223,48 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (even CTA)
-    if (leader && lane == 0) {
+    if (leader) {  // the whole warp runs the loop, one lane issues: operands stay in uniform registers
       constexpr uint32_t IDESC = idesc_bf16_f32(2 * BM, 256, false, kDz);
+      const uint64_t a0 = smem_desc_sw128(smem_u32(sA), 16, 1024);
+      const uint64_t b0 = kDz ? smem_desc_sw128(smem_u32(sB), 8192, 1024) : smem_desc_sw128(smem_u32(sB), 16, 1024);
+      auto ready = [&](uint64_t* bar, uint32_t parity) -> bool {
+        const bool now = mbar_try_wait(bar, parity) || (*abort_flag == 0 && mbar_wait(bar, parity, p.timeout_ns));
+        return __all_sync(0xffffffffu, now);
+      };
       int stage = 0, local = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int u = cluster; ok && u < p.num_units; u += clusters, ++local) {
         const int acc = local & 1;
-        if (*abort_flag || !mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, p.timeout_ns)) {
-          report_status(p.status, kStatusTimeoutMma);
-          *abort_flag = 1;
-          break;
-        }
+        ok = ready(&tempty[acc], ((local >> 1) & 1) ^ 1);
+        if (!ok) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * 256);
         for (int kb = 0; kb < k_blocks; ++kb) {
-          if (*abort_flag || !mbar_wait(&full[stage], phase, p.timeout_ns)) {
-            report_status(p.status, kStatusTimeoutMma);
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
+          ok = ready(&full[stage], phase);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t a = smem_u32(sA + stage * kTile), b = smem_u32(sB + stage * kTile);
+          const uint64_t a = a0 + static_cast<uint32_t>(stage * (kTile >> 4));
+          const uint64_t b = b0 + static_cast<uint32_t>(stage * (kTile >> 4));
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk)
-            umma_f16_ss_pair(d_tmem, smem_desc_sw128(a + kk * 32, 16, 1024),
-                             kDz ? smem_desc_sw128(b + kk * 2048, 8192, 1024)
-                                       : smem_desc_sw128(b + kk * 32, 16, 1024),
-                             IDESC, (kb > 0 || kk > 0) ? 1u : 0u);
-          umma_commit_pair(&empty[stage], 0x3);
+            for (int kk = 0; kk < BK / 16; ++kk)
+              umma_f16_ss_pair(d_tmem, a + kk * 2, b + kk * (kDz ? 128 : 2), IDESC, (kb > 0 || kk > 0) ? 1u : 0u);
+            umma_commit_pair(&empty[stage], 0x3);
+            if (kb + 1 == k_blocks) umma_commit_pair(&tfull[acc], 0x3);
+          }
+          __syncwarp();
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1;
           }
         }
-        if (!ok) break;
-        umma_commit_pair(&tfull[acc], 0x3);
       }
-      umma_commit_pair(drain, 0x3);
+      if (!ok) {
+        if (lane == 0) report_status(p.status, kStatusTimeoutMma);
+        *abort_flag = 1;
+      }
+      if (elect_one()) umma_commit_pair(drain, 0x3);
     }
     if (lane == 0 && !mbar_wait(drain, 0, p.timeout_ns)) report_status(p.status, kStatusTimeoutDrain);
     __syncwarp();
@@ -359,13 +363,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if constexpr (kSave) {
             float b[32];
             float top_a = 0.f, top_b = 0.f;
+gate_and_keep(p.act, g, v, b);
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              float value, grad;
-              act_value_grad(g[i], p.act, value, grad);
-              g[i] = value;
-              b[i] = v[i] * grad;
-              v[i] *= value;
               top_a = fmaxf(top_a, fabsf(g[i]));
               top_b = fmaxf(top_b, fabsf(b[i]));
             }
@@ -381,8 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             stage_half32(buf, lane, g, store_factor(ea));
             staging.store(&tmOut2, buf, n, row0, lane);
           } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= act_value(g[i], p.act);
+            gate(p.act, g, v);
             uint8_t* buf = staging.next(lane);
             gemm::stage_row32_sw64(buf, lane, v);
             staging.store(&tmOut0, buf, n, row0, lane);

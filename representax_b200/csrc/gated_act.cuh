@@ -17,39 +17,70 @@ namespace gated {
 
 enum Act : int { kGeluErf = 0, kGeluTanh = 1, kSilu = 2, kQuickGelu = 3 };
 
+template <int ACT>
+struct ActCode {
+  static constexpr int value = ACT;
+};
+
 __device__ __forceinline__ float logistic(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
-__device__ __forceinline__ float act_value(float g, int act) {
-  switch (act) {
-    case kGeluErf: return gemm::gelu_erf(g);
-    case kGeluTanh: return g * logistic(1.5957691216057308f * fmaf(0.044715f * g * g, g, g));
-    case kSilu: return g * logistic(g);
-    default: return g * logistic(1.702f * g);
+template <int ACT>
+__device__ __forceinline__ float act_value(float g) {
+  if constexpr (ACT == kGeluErf) return gemm::gelu_erf(g);
+  if constexpr (ACT == kGeluTanh) return g * logistic(1.5957691216057308f * fmaf(0.044715f * g * g, g, g));
+  if constexpr (ACT == kSilu) return g * logistic(g);
+  return g * logistic(1.702f * g);
+}
+
+template <int ACT>
+__device__ __forceinline__ void act_value_grad(float g, float& value, float& grad) {
+  if constexpr (ACT == kGeluErf) {
+    gemm::gelu_and_grad(g, value, grad);
+  } else if constexpr (ACT == kGeluTanh) {
+    const float s = logistic(1.5957691216057308f * fmaf(0.044715f * g * g, g, g));
+    value = g * s;
+    grad = fmaf(g * s * (1.f - s), 1.5957691216057308f * fmaf(0.134145f * g, g, 1.f), s);
+  } else {
+    constexpr float k = ACT == kSilu ? 1.f : 1.702f;
+    const float s = logistic(k * g);
+    value = g * s;
+    grad = fmaf(k * g * s, 1.f - s, s);
   }
 }
 
-__device__ __forceinline__ void act_value_grad(float g, int act, float& value, float& grad) {
+// f(integral_constant of the activation): the choice is made once for a run of values, not for each.
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F&& f) {
   switch (act) {
-    case kGeluErf: gemm::gelu_and_grad(g, value, grad); return;
-    case kGeluTanh: {
-      const float s = logistic(1.5957691216057308f * fmaf(0.044715f * g * g, g, g));
-      value = g * s;
-      grad = fmaf(g * s * (1.f - s), 1.5957691216057308f * fmaf(0.134145f * g, g, 1.f), s);
-      return;
-    }
-    case kSilu: {
-      const float s = logistic(g);
-      value = g * s;
-      grad = fmaf(g * s, 1.f - s, s);
-      return;
-    }
-    default: {
-      const float s = logistic(1.702f * g);
-      value = g * s;
-      grad = fmaf(1.702f * g * s, 1.f - s, s);
-      return;
-    }
+    case kGeluErf: f(ActCode<kGeluErf>{}); return;
+    case kGeluTanh: f(ActCode<kGeluTanh>{}); return;
+    case kSilu: f(ActCode<kSilu>{}); return;
+    default: f(ActCode<kQuickGelu>{}); return;
   }
+}
+
+// v[i] = act(g[i]) * v[i]
+template <int N>
+__device__ __forceinline__ void gate(int act, const float (&g)[N], float (&v)[N]) {
+  with_act(act, [&](auto code) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] *= act_value<decltype(code)::value>(g[i]);
+  });
+}
+
+// a = act(g), b = act'(g) * u, u becomes act(g) * u (g holds a afterwards)
+template <int N>
+__device__ __forceinline__ void gate_and_keep(int act, float (&g)[N], float (&u)[N], float (&b)[N]) {
+  with_act(act, [&](auto code) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float value, grad;
+      act_value_grad<decltype(code)::value>(g[i], value, grad);
+      g[i] = value;
+      b[i] = u[i] * grad;
+      u[i] *= value;
+    }
+  });
 }
 
 }  // namespace gated
