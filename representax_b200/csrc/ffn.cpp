@@ -44,12 +44,17 @@ void check_sizes(int64_t T, int64_t H, int64_t I) {
   RX_CHECK(T < (1ll << 31) - 256 && H < (1ll << 30) && I < (1ll << 30), "gated feed-forward too large");
 }
 
+int64_t saved_tiles(int64_t T, int64_t I) { return (T + 31) / 32 * ((I + 31) / 32); }
+
+// What the forward keeps (gated.h): fp16 [tiles, 2, 32, 32] and int16 [tiles, 32].
 void check_saved(const at::Tensor& saved, const at::Tensor& exps, int64_t T, int64_t I, int device) {
-  RX_CHECK(saved.scalar_type() == at::kHalf, "saved must be float16");
-  check_rows(saved, "saved", T, 2 * I, device);
+  const int64_t tiles = saved_tiles(T, I);
+  RX_CHECK(saved.is_cuda() && saved.get_device() == device && saved.scalar_type() == at::kHalf && saved.is_contiguous() &&
+               saved.numel() == tiles * 2048 && reinterpret_cast<uintptr_t>(saved.data_ptr()) % 16 == 0,
+           "saved must be a contiguous float16 array of ", tiles * 2048);
   RX_CHECK(exps.is_cuda() && exps.get_device() == device && exps.scalar_type() == at::kShort && exps.is_contiguous() &&
-               exps.dim() == 2 && exps.size(0) == T && exps.size(1) == (I + 31) / 32,
-           "exps must be a contiguous int16 [T, ceil(I / 32)]");
+               exps.numel() == tiles * 32,
+           "exps must be a contiguous int16 array of ", tiles * 32);
 }
 
 gated::Params make_params(int64_t T, int64_t I, int64_t H, int64_t tile_cols, const at::Tensor& status) {
@@ -167,8 +172,7 @@ void few_rows_linear(const at::Tensor& x, const at::Tensor& w, int64_t parts, in
 }
 
 // h [T, I] = act(x Wg^T + bg) * (x Wu^T + bu) for x [T, H] and gate_up = [Wg; Wu] [2 I, H].
-// With `saved` (fp16 [T, 2 I]: b, then a) and `exps` (int16 [T, ceil(I / 32)]) it also keeps what
-// gated_backward reads.
+// With `saved` and `exps` (see check_saved) it also keeps what gated_backward reads.
 void gated_forward(const at::Tensor& x, const at::Tensor& gate_up, const OptTensor& bias, at::Tensor& h,
                    const OptTensor& saved, const OptTensor& exps, int64_t act, const at::Tensor& status) {
   check_bf16(x, "x");
@@ -196,17 +200,15 @@ void gated_forward(const at::Tensor& x, const at::Tensor& gate_up, const OptTens
   gated::Maps maps;
   maps.a = make_tmap_2d_bf16(x.data_ptr(), T, H, x.stride(0), 64, 128);
   maps.b = make_tmap_2d_bf16(gate_up.data_ptr(), 2 * I, H, gate_up.stride(0), 64, 128);
-  maps.out[0] = maps.out[1] = maps.out[2] = make_tmap_2d_bf16_store(h.data_ptr(), T, I, h.stride(0));
+  p.out[0] = reinterpret_cast<__nv_bfloat16*>(h.data_ptr());
+  p.ld_out = h.stride(0);
   if (!saved.has_value()) {
     run(gated::kForward, maps, p, dev);
     return;
   }
   check_saved(*saved, *exps, T, I, dev);
   p.exps = reinterpret_cast<uint16_t*>(exps->data_ptr());
-  p.ld_exps = exps->size(1);
-  auto* sp = reinterpret_cast<__half*>(saved->data_ptr());
-  maps.out[1] = make_tmap_2d_bf16_store(sp, T, I, saved->stride(0));
-  maps.out[2] = make_tmap_2d_bf16_store(sp + I, T, I, saved->stride(0));
+  p.saved = reinterpret_cast<uint4*>(saved->data_ptr());
   run(gated::kForwardSave, maps, p, dev);
 }
 
@@ -225,18 +227,16 @@ void gated_backward(const at::Tensor& dy, const at::Tensor& down, const at::Tens
   check_rows(dz, "dz", T, 2 * I, dev);
   check_saved(saved, exps, T, I, dev);
   gated::Params p = make_params(T, I, H, 256, status);
-  p.saved_b = reinterpret_cast<const __half*>(saved.data_ptr());
-  p.saved_a = p.saved_b + I;
-  p.ld_saved = saved.stride(0);
+  p.saved = reinterpret_cast<uint4*>(saved.data_ptr());
   p.exps = reinterpret_cast<uint16_t*>(exps.data_ptr());
-  p.ld_exps = exps.size(1);
   c10::cuda::CUDAGuard guard(dev);
   auto* zp = reinterpret_cast<__nv_bfloat16*>(dz.data_ptr());
   gated::Maps maps;
   maps.a = make_tmap_2d_bf16(dy.data_ptr(), T, H, dy.stride(0), 64, 128);
   maps.b = make_tmap_2d_bf16(down.data_ptr(), H, I, down.stride(0), 64, 64);
-  maps.out[0] = make_tmap_2d_bf16_store(zp, T, I, dz.stride(0));
-  maps.out[1] = maps.out[2] = make_tmap_2d_bf16_store(zp + I, T, I, dz.stride(0));
+  p.out[0] = zp;
+  p.out[1] = zp + I;
+  p.ld_out = dz.stride(0);
   run(gated::kBackward, maps, p, dev);
 }
 
@@ -257,8 +257,8 @@ std::vector<at::Tensor> gated_ffn_forward(const at::Tensor& x_in, const at::Tens
   at::Tensor h = at::empty({T, I}, x.options()), y = at::empty({T, H}, x.options()), saved, exps;
   const bool few = T <= few::kMaxRows;
   if (save) {
-    saved = at::empty({T, 2 * I}, x.options().dtype(at::kHalf));
-    exps = at::empty({T, (I + 31) / 32}, x.options().dtype(at::kShort));
+    saved = at::empty({saved_tiles(T, I), 2, 32, 32}, x.options().dtype(at::kHalf));
+    exps = at::empty({saved_tiles(T, I), 32}, x.options().dtype(at::kShort));
     gated_forward(x, gate_up, b1, h, saved, exps, act, status);
   } else if (few) {
     few_rows_linear(x, gate_up, 2, act, b1, c10::nullopt, h, false, status);

@@ -18,15 +18,18 @@
 // epilogue that produces dz only multiplies: dz = [dh b | dh a]. Both are kept
 // as fp16 with one power of two per row and 32 columns (an exponent byte that
 // puts the block's largest value into [2^14, 2^15)): 11 significant bits down to
-// 2^-29 of that value for the bytes of bf16's 8 bits, so the rounding of dz to bf16 (which the
-// tensor core needs) stays the only one that counts.
+// 2^-29 of that value in the bytes of bf16's 8 bits, so the rounding of dz to bf16
+// (which the tensor core needs) stays the only one that counts. They are laid
+// out as 32 x 32 tiles of 2 KB, b and a side by side, in the order in which the
+// lanes of a warp write and read them: whole cache lines, and no detour through
+// shared memory. (Row-major, the 64-byte pieces of 32 rows were slower in both passes.)
 //
 // Backward: the input-gradient GEMM dy Wd with 256 x 256 pair tiles whose
 // epilogue reads the saved tiles (prefetched one 32-column chunk ahead) and
 // stores the two halves of dz; dh is never written.
 //
 // Both are bound by the tensor pipe at training sizes (see the figures at the
-// host entries). The main loops follow the pair kernel of gemm_kernel.cuh: six
+// host entries). The main loops follow the pair kernel of gemm_kernel.cuh: five
 // 32 KB stages, TMA with the 128-byte swizzle, one issuing thread, two
 // accumulator buffers so that an epilogue overlaps the next tile's products.
 #include "gated.h"
@@ -49,7 +52,7 @@ constexpr int kThreads = 64 + 32 * kEpilogueWarps;
 
 constexpr int kStages = 6;
 constexpr int kTile = BM * BK * 2;  // 16 KB: 128 rows x 64 bf16
-constexpr int kStaging = kEpilogueWarps * 2 * 2048;
+constexpr int kStaging = kEpilogueWarps * 2048;  // a 32 x 32 tile of 16-bit values for each epilogue warp
 constexpr size_t kSmem = 1024 + kStages * 2 * kTile + kStaging + 256;
 static_assert(kSmem <= 232448, "shared memory beyond the opt-in limit");
 
@@ -62,50 +65,49 @@ __device__ __forceinline__ uint32_t block_byte(float top) {
 __device__ __forceinline__ float store_factor(uint32_t e) { return __uint_as_float((268u - e) << 23); }
 __device__ __forceinline__ float load_factor(uint32_t e) { return __uint_as_float((e - 14u) << 23); }
 
-// Row `lane` of a 32 x 32 tile of 16-bit values staged for a tile store (64-byte swizzle).
-__device__ __forceinline__ void stage_half32(uint8_t* buf, int lane, const float (&v)[32], float f) {
+// A lane's row of a saved 32 x 32 tile: four 16-byte pieces, piece q of all lanes together.
+__device__ __forceinline__ void save_row32(uint4* tile, int lane, const float (&v)[32], float f) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     uint4 w;
     __half2* h = reinterpret_cast<__half2*>(&w);
 #pragma unroll
     for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(v[q * 8 + 2 * j] * f, v[q * 8 + 2 * j + 1] * f);
-    *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16)) = w;
+    tile[q * 32 + lane] = w;
   }
 }
-__device__ __forceinline__ void read_half32(const uint8_t* buf, int lane, float (&v)[32], float f) {
+__device__ __forceinline__ void fetch_row32(const uint4* tile, int lane, uint4 (&w)[4]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) w[q] = ldg_v4_issue(tile + q * 32 + lane);
+}
+// v[i] = saved value i * f * r[i]
+__device__ __forceinline__ void times_row32(const uint4 (&w)[4], float f, const uint32_t (&r)[32], float (&v)[32]) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const uint4 w = *reinterpret_cast<const uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16));
-    const __half2* h = reinterpret_cast<const __half2*>(&w);
+    const __half2* h = reinterpret_cast<const __half2*>(&w[q]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 t = __half22float2(h[j]);
-      v[q * 8 + 2 * j] = t.x * f;
-      v[q * 8 + 2 * j + 1] = t.y * f;
+      v[q * 8 + 2 * j] = t.x * f * __uint_as_float(r[q * 8 + 2 * j]);
+      v[q * 8 + 2 * j + 1] = t.y * f * __uint_as_float(r[q * 8 + 2 * j + 1]);
     }
   }
 }
 
-// One warp's staged stores: two 2 KB buffers used in turn; a buffer is free
-// once at most one of the lane's committed stores is still reading.
-struct Staging {
-  uint8_t* base;
-  uint32_t seq = 0;
-  __device__ __forceinline__ uint8_t* next(int lane) {
-    if (lane == 0) tma_store_wait_read<1>();
-    __syncwarp();
-    return base + (seq++ & 1) * 2048;
+// A warp's 32 x 32 tile of 16-bit values from its staging buffer to rows row0.. and columns n.. of a
+// matrix: 16-byte pieces, four lanes to a 64-byte row segment.
+__device__ __forceinline__ void store_tile32(const uint8_t* buf, __nv_bfloat16* dst, int64_t ld, int row0, int n, int rows, int cols,
+                                             int lane) {
+  __syncwarp();
+#pragma unroll
+  for (int it = 0; it < 4; ++it) {
+    const int c = lane + 32 * it, row = c >> 2, piece = c & 3;
+    const uint4 w = *reinterpret_cast<const uint4*>(buf + row * 64 + ((piece ^ ((row >> 1) & 3)) * 16));
+    if (row0 + row < rows && n + piece * 8 < cols)
+      *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(row0 + row) * ld + n + piece * 8) = w;
   }
-  __device__ __forceinline__ void store(const CUtensorMap* map, const uint8_t* buf, int x, int y, int lane) {
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      tma_store_2d(map, buf, x, y);
-      tma_store_commit();
-    }
-  }
-};
+  __syncwarp();
+}
 
 __device__ __forceinline__ void add_bias32(const __nv_bfloat16* bias, int n_base, int n, float (&v)[32]) {
   if (n_base + 32 <= n) {
@@ -119,11 +121,14 @@ __device__ __forceinline__ void add_bias32(const __nv_bfloat16* bias, int n_base
   }
 }
 
+// Index of the saved tile that holds rows row0.. (of 32) and columns n.. (of 32).
+__device__ __forceinline__ int64_t tile_of(const Params& p, int row0, int n) {
+  return static_cast<int64_t>(row0 >> 5) * ((p.N + 31) >> 5) + (n >> 5);
+}
+
 template <int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
-    gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                 const __grid_constant__ CUtensorMap tmOut0, const __grid_constant__ CUtensorMap tmOut1,
-                 const __grid_constant__ CUtensorMap tmOut2, const Params p) {
+    gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
   constexpr bool kDz = MODE == kBackward;
   constexpr bool kSave = MODE == kForwardSave;
   constexpr int kTileCols = kDz ? 256 : 128;  // output columns of a tile
@@ -163,7 +168,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0 && lane == 0) {
     tma_prefetch_map(&tmA);
     tma_prefetch_map(&tmB);
-    tma_prefetch_map(&tmOut0);
   }
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, kTmemCols);
@@ -274,23 +278,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kChunks = kTileCols / 32 / (kEpilogueWarps / 4);
     const int chunk0 = ((warp - 2) / 4) * kChunks;
     const uint32_t tempty_leader = mapa_shared(smem_u32(&tempty[0]), 0);
-    Staging staging{sC + (warp - 2) * 4096};
+    uint8_t* const buf = sC + (warp - 2) * 2048;
     int local = 0;
     for (int u = cluster; u < p.num_units; u += clusters, ++local) {
       const int acc = local & 1;
       const int row0 = (u / p.n_tiles) * (2 * BM) + rank * BM + quad * 32;  // this warp's 32 rows
       const int n0 = (u % p.n_tiles) * kTileCols;
-      const int m = row0 + lane;
       uint4 next_b[4], next_a[4];
       uint32_t next_e = 0;
-      if constexpr (kDz) {  // the first chunk's saved tiles, in flight while the products finish
+      if constexpr (kDz) {
         const int n = n0 + chunk0 * 32;
         if (n < p.N && row0 < p.M) {
-          gemm::warp_fetch_tile32(reinterpret_cast<const __nv_bfloat16*>(p.saved_b), p.ld_saved, row0, n, p.M, p.N, lane,
-                                  next_b);
-          gemm::warp_fetch_tile32(reinterpret_cast<const __nv_bfloat16*>(p.saved_a), p.ld_saved, row0, n, p.M, p.N, lane,
-                                  next_a);
-          if (m < p.M) next_e = p.exps[static_cast<int64_t>(m) * p.ld_exps + (n >> 5)];
+          const int64_t t = tile_of(p, row0, n);
+          fetch_row32(p.saved + t * 256, lane, next_b);
+          fetch_row32(p.saved + t * 256 + 128, lane, next_a);
+          next_e = p.exps[t * 32 + lane];
         }
       }
       bool ok = (*abort_flag == 0) && mbar_wait(&tfull[acc], (local >> 1) & 1, p.timeout_ns);
@@ -317,27 +319,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             cur_a[q] = next_a[q];
           }
           if (c + 1 < chunk0 + kChunks && n + 32 < p.N && row0 < p.M) {
-            gemm::warp_fetch_tile32(reinterpret_cast<const __nv_bfloat16*>(p.saved_b), p.ld_saved, row0, n + 32, p.M, p.N,
-                                    lane, next_b);
-            gemm::warp_fetch_tile32(reinterpret_cast<const __nv_bfloat16*>(p.saved_a), p.ld_saved, row0, n + 32, p.M, p.N,
-                                    lane, next_a);
-            if (m < p.M) next_e = p.exps[static_cast<int64_t>(m) * p.ld_exps + ((n + 32) >> 5)];
+            const int64_t t = tile_of(p, row0, n + 32);
+            fetch_row32(p.saved + t * 256, lane, next_b);
+            fetch_row32(p.saved + t * 256 + 128, lane, next_a);
+            next_e = p.exps[t * 32 + lane];
           }
           tmem_ld_wait();
           if (!live) continue;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            uint8_t* buf = staging.next(lane);
             float v[32];
-            gemm::warp_put_tile32_sw64(buf, lane, half == 0 ? cur_b : cur_a);
-            __syncwarp();
-            // rows past the end hold zeros and an exponent byte that reads as the smallest factor
-            read_half32(buf, lane, v, load_factor(max(half == 0 ? e & 0xffu : e >> 8, 15u)));
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= __uint_as_float(r[i]);
+            if (half == 0)
+              times_row32(cur_b, load_factor(e & 0xffu), r, v);
+            else
+              times_row32(cur_a, load_factor(e >> 8), r, v);
             gemm::stage_row32_sw64(buf, lane, v);
-            staging.store(half == 0 ? &tmOut0 : &tmOut1, buf, n, row0, lane);
+            store_tile32(buf, p.out[half], p.ld_out, row0, n, p.M, p.N, lane);
           }
         } else {
           uint32_t rg[32], ru[32];
@@ -370,21 +367,16 @@ gate_and_keep(p.act, g, v, b);
               top_b = fmaxf(top_b, fabsf(b[i]));
             }
             const uint32_t ea = block_byte(top_a), eb = block_byte(top_b);
-            if (m < p.M) p.exps[static_cast<int64_t>(m) * p.ld_exps + (n >> 5)] = static_cast<uint16_t>(eb | (ea << 8));
-            uint8_t* buf = staging.next(lane);
+            const int64_t t = tile_of(p, row0, n);
+            p.exps[t * 32 + lane] = static_cast<uint16_t>(eb | (ea << 8));
+            save_row32(p.saved + t * 256, lane, b, store_factor(eb));
+            save_row32(p.saved + t * 256 + 128, lane, g, store_factor(ea));
             gemm::stage_row32_sw64(buf, lane, v);
-            staging.store(&tmOut0, buf, n, row0, lane);
-            buf = staging.next(lane);
-            stage_half32(buf, lane, b, store_factor(eb));
-            staging.store(&tmOut1, buf, n, row0, lane);
-            buf = staging.next(lane);
-            stage_half32(buf, lane, g, store_factor(ea));
-            staging.store(&tmOut2, buf, n, row0, lane);
+            store_tile32(buf, p.out[0], p.ld_out, row0, n, p.M, p.N, lane);
           } else {
             gate(p.act, g, v);
-            uint8_t* buf = staging.next(lane);
             gemm::stage_row32_sw64(buf, lane, v);
-            staging.store(&tmOut0, buf, n, row0, lane);
+            store_tile32(buf, p.out[0], p.ld_out, row0, n, p.M, p.N, lane);
           }
         }
       }
@@ -392,8 +384,6 @@ gate_and_keep(p.act, g, v, b);
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(tempty_leader + acc * 8);
     }
-    if (lane == 0) tma_store_wait<0>();  // every tile store has landed before the CTA exits
-    __syncwarp();
   }
 
   tc_fence_before();
@@ -424,7 +414,7 @@ cudaError_t launch_mode(const Maps& maps, const Params& p, int sms, int device, 
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, maps.a, maps.b, maps.out[0], maps.out[1], maps.out[2], p);
+  return cudaLaunchKernelEx(&cfg, kern, maps.a, maps.b, p);
 }
 
 cudaError_t launch(int mode, const Maps& maps, const Params& p, int sms, int device, cudaStream_t stream) {

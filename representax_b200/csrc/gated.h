@@ -2,7 +2,6 @@
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -17,19 +16,17 @@ struct Params {
   int m_tiles, n_tiles, num_units;
   int act;
   const __nv_bfloat16* bias;  // forward: [2 N] (gate, up) or null
-  const __half* saved_b;      // backward: b [M, N], a [M, N] with row stride ld_saved
-  const __half* saved_a;
-  int64_t ld_saved;
-  uint16_t* exps;             // [M, ceil(N / 32)]: low byte the block exponent of b, high byte that of a
-  int64_t ld_exps;
+  __nv_bfloat16* out[2];      // h (forward) or the two halves of dz, [M, N]
+  int64_t ld_out;
+  uint4* saved;               // [ceil(M / 32)][ceil(N / 32)] tiles of 32 x 32 fp16: b, then a (4 KB)
+  uint16_t* exps;             // [the same tiles][32]: low byte the block exponent of b, high byte that of a
   int* status;
   uint64_t timeout_ns;
 };
 
-// a: boxes of 128 rows x 64; b: 128 x 64 (forward, K-major) or 64 x 64 (backward, MN-major);
-// out: 32 x 32 store maps of h, b, a (forward) or of the two halves of dz.
+// a: boxes of 128 rows x 64; b: 128 x 64 (forward, K-major) or 64 x 64 (backward, MN-major).
 struct Maps {
-  CUtensorMap a, b, out[3];
+  CUtensorMap a, b;
 };
 
 cudaError_t launch(int mode, const Maps& maps, const Params& p, int sms, int device, cudaStream_t stream);
