@@ -35,7 +35,11 @@ namespace fp4 {
 constexpr int kTile = 128 * 128;   // 128 rows x 256 codes
 constexpr int kGemmStages = 5;
 constexpr int kEpiWarps = 8;
-constexpr int kGemmThreads = 32 * (2 + kEpiWarps);
+constexpr int kFirstEpi = 4;  // warps 0 (producer) and 1 (MMA issuer) share a warpgroup with two idle ones
+constexpr int kGemmThreads = 32 * (kFirstEpi + kEpiWarps);
+// Registers of the two roles: an epilogue thread holds 128 accumulators. 128 * 64 + 256 * 216 is below the
+// 384 * 168 that the block is launched with.
+constexpr int kIssueRegs = 64, kEpiRegs = 216;
 constexpr int kStaging = kEpiWarps * 2 * 2048;
 
 template <int FMT>
@@ -159,6 +163,131 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
   const int num_units = p.m_tiles * p.n_tiles;
 
+  if (warp >= kFirstEpi) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
+    // ------------------------------------------------------------ epilogue (both CTAs)
+    const int quad = warp & 3, half = (warp - kFirstEpi) >> 2;
+    const uint32_t tempty_leader = mapa_shared(smem_u32(tempty), 0);
+    uint8_t* const staging = sC + (warp - kFirstEpi) * 4096;
+    int local = 0;
+    uint32_t seq = 0;
+    for (int u = cluster; u < num_units; u += clusters, ++local) {
+      const int mt = u % p.m_tiles, nt = u / p.m_tiles;
+      const int row0 = mt * 256 + rank * 128 + quad * 32;  // this warp's 32 rows
+      uint4 next[4];  // the next chunk's residual tile, in flight
+      const bool side = !GATED && p.residual != nullptr && p.vec && row0 < p.M;
+      if (side && nt * kTileN + half * 128 < p.N)
+        gemm::warp_fetch_tile32(p.residual, p.ld_res, row0, nt * kTileN + half * 128, p.M, p.N, lane, next);
+      bool ok = (*abort_flag == 0) && mbar_wait(tfull, local & 1, p.timeout_ns);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        if (lane == 0) report_status(p.status, kStatusTimeoutEpilogue);
+        *abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      // plain: 128 columns of this half; gated: 64 gate columns, then the 64 up columns of the same outputs
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+      uint32_t r[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        tmem_ld_32x32b_x32(t_row + (GATED ? half * 64 + (c & 1) * 32 + (c >> 1) * 128 : half * 128 + c * 32), r[c]);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(tempty_leader);
+      if (row0 >= p.M) continue;  // warp-uniform
+      const int64_t m = row0 + lane;
+      const bool live = m < p.M;
+      const float row_a = FMT == kNv && live ? p.row_a[m] : 1.f;
+      // 32 outputs of every row of the warp, from column n
+      auto put = [&](int n, float (&v)[32], const uint4* res) {
+        if (!p.vec) {
+          if (live) store32(p, m, n, v);
+          return;
+        }
+        uint8_t* buf = staging + (seq++ & 1) * 2048;
+        if (lane == 0) tma_store_wait_read<1>();  // the store that last read `buf` is done reading
+        __syncwarp();
+        if (res != nullptr) {  // the tile's rows to their threads
+          float add[32];
+          gemm::warp_put_tile32_sw64(buf, lane, *reinterpret_cast<const uint4(*)[4]>(res));
+          __syncwarp();
+          gemm::read_row32_sw64(buf, lane, add);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += add[i];
+        }
+        gemm::stage_row32_sw64(buf, lane, v);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&tmOut, buf, n, row0);
+          tma_store_commit();
+        }
+      };
+      if constexpr (GATED) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int n = nt * kTileN + half * 64 + c * 32;
+          // (a quantised output also defines the blocks past N of the tile)
+          if (n >= p.N && p.q_out == nullptr) continue;
+          float g[32], v[32];
+          finish32<FMT>(p, row_a, 0, n, r[c], g);
+          finish32<FMT>(p, row_a, p.N, n, r[2 + c], v);
+          gated::gate(p.act, g, v);
+          if (FMT == kMx && p.q_out != nullptr) {
+            if (!live) continue;
+            if (n + 32 > p.N) {  // columns past the end: zeros in the next layer's contraction
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (n + i >= p.N) v[i] = 0.f;
+            }
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+            const uint32_t byte = mx_scale_byte(top);
+            const float inv = mx_inverse(byte);
+            uint32_t codes[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float w[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) w[i] = v[8 * q + i] * inv;
+              codes[q] = pack8(w);
+            }
+            if ((n >> 1) < p.ld_q)
+              *reinterpret_cast<uint4*>(p.q_out + m * p.ld_q + (n >> 1)) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+            p.q_sf[scale_offset(m, n >> 5, p.q_groups)] = static_cast<uint8_t>(byte);
+          } else {
+            put(n, v, nullptr);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int n = nt * kTileN + half * 128 + c * 32;
+          if (n >= p.N) continue;
+          float v[32];
+          finish32<FMT>(p, row_a, 0, n, r[c], v);
+          if (side) {
+            uint4 cur[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) cur[q] = next[q];
+            if (c < 3 && n + 32 < p.N)
+              gemm::warp_fetch_tile32(p.residual, p.ld_res, row0, n + 32, p.M, p.N, lane, next);
+            put(n, v, cur);
+          } else {
+            if (p.residual != nullptr && live) add32(p.residual + m * p.ld_res + n, false, n, p.N, v);
+            put(n, v, nullptr);
+          }
+        }
+      }
+    }
+    if (lane == 0) tma_store_wait<0>();  // every tile store has landed before the CTA exits
+    __syncwarp();
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
@@ -289,128 +418,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     }
     if (lane == 0 && !mbar_wait(drain, 0, p.timeout_ns)) report_status(p.status, kStatusTimeoutDrain);
     __syncwarp();
-  } else {
-    // ------------------------------------------------------------ epilogue (both CTAs)
-    const int quad = warp & 3, half = (warp - 2) >> 2;
-    const uint32_t tempty_leader = mapa_shared(smem_u32(tempty), 0);
-    uint8_t* const staging = sC + (warp - 2) * 4096;
-    int local = 0;
-    uint32_t seq = 0;
-    for (int u = cluster; u < num_units; u += clusters, ++local) {
-      const int mt = u % p.m_tiles, nt = u / p.m_tiles;
-      const int row0 = mt * 256 + rank * 128 + quad * 32;  // this warp's 32 rows
-      uint4 next[4];  // the next chunk's residual tile, in flight
-      const bool side = !GATED && p.residual != nullptr && p.vec && row0 < p.M;
-      if (side && nt * kTileN + half * 128 < p.N)
-        gemm::warp_fetch_tile32(p.residual, p.ld_res, row0, nt * kTileN + half * 128, p.M, p.N, lane, next);
-      bool ok = (*abort_flag == 0) && mbar_wait(tfull, local & 1, p.timeout_ns);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) {
-        if (lane == 0) report_status(p.status, kStatusTimeoutEpilogue);
-        *abort_flag = 1;
-        break;
-      }
-      tc_fence_after();
-      // plain: 128 columns of this half; gated: 64 gate columns, then the 64 up columns of the same outputs
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
-      uint32_t r[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        tmem_ld_32x32b_x32(t_row + (GATED ? half * 64 + (c & 1) * 32 + (c >> 1) * 128 : half * 128 + c * 32), r[c]);
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(tempty_leader);
-      if (row0 >= p.M) continue;  // warp-uniform
-      const int64_t m = row0 + lane;
-      const bool live = m < p.M;
-      const float row_a = FMT == kNv && live ? p.row_a[m] : 1.f;
-      // 32 outputs of every row of the warp, from column n
-      auto put = [&](int n, float (&v)[32], const uint4* res) {
-        if (!p.vec) {
-          if (live) store32(p, m, n, v);
-          return;
-        }
-        uint8_t* buf = staging + (seq++ & 1) * 2048;
-        if (lane == 0) tma_store_wait_read<1>();  // the store that last read `buf` is done reading
-        __syncwarp();
-        if (res != nullptr) {  // the tile's rows to their threads
-          float add[32];
-          gemm::warp_put_tile32_sw64(buf, lane, *reinterpret_cast<const uint4(*)[4]>(res));
-          __syncwarp();
-          gemm::read_row32_sw64(buf, lane, add);
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] += add[i];
-        }
-        gemm::stage_row32_sw64(buf, lane, v);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_2d(&tmOut, buf, n, row0);
-          tma_store_commit();
-        }
-      };
-      if constexpr (GATED) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int n = nt * kTileN + half * 64 + c * 32;
-          // (a quantised output also defines the blocks past N of the tile)
-          if (n >= p.N && p.q_out == nullptr) continue;
-          float g[32], v[32];
-          finish32<FMT>(p, row_a, 0, n, r[c], g);
-          finish32<FMT>(p, row_a, p.N, n, r[2 + c], v);
-          gated::gate(p.act, g, v);
-          if (FMT == kMx && p.q_out != nullptr) {
-            if (!live) continue;
-            if (n + 32 > p.N) {  // columns past the end: zeros in the next layer's contraction
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (n + i >= p.N) v[i] = 0.f;
-            }
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-            const uint32_t byte = mx_scale_byte(top);
-            const float inv = mx_inverse(byte);
-            uint32_t codes[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float w[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) w[i] = v[8 * q + i] * inv;
-              codes[q] = pack8(w);
-            }
-            if ((n >> 1) < p.ld_q)
-              *reinterpret_cast<uint4*>(p.q_out + m * p.ld_q + (n >> 1)) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-            p.q_sf[scale_offset(m, n >> 5, p.q_groups)] = static_cast<uint8_t>(byte);
-          } else {
-            put(n, v, nullptr);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int n = nt * kTileN + half * 128 + c * 32;
-          if (n >= p.N) continue;
-          float v[32];
-          finish32<FMT>(p, row_a, 0, n, r[c], v);
-          if (side) {
-            uint4 cur[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) cur[q] = next[q];
-            if (c < 3 && n + 32 < p.N)
-              gemm::warp_fetch_tile32(p.residual, p.ld_res, row0, n + 32, p.M, p.N, lane, next);
-            put(n, v, cur);
-          } else {
-            if (p.residual != nullptr && live) add32(p.residual + m * p.ld_res + n, false, n, p.N, v);
-            put(n, v, nullptr);
-          }
-        }
-      }
-    }
-    if (lane == 0) tma_store_wait<0>();  // every tile store has landed before the CTA exits
-    __syncwarp();
+  }
   }
 
   tc_fence_before();

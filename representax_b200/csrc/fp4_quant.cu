@@ -15,9 +15,9 @@
 // the scales are written; the instructions per value are the next limit, so
 //  * a lane takes 8 consecutive values (one or two 16-byte loads, one 4-byte
 //    store) and a warp 256; maxima are taken on the raw 16-bit pairs;
-//  * a warp has up to kKeep such pieces of its row in flight and keeps them
-//    in registers, so NVFP4 has the row's maximum before it codes without a
-//    second read (rows beyond 8 warps * kKeep pieces are read twice);
+//  * a warp has kAhead such pieces of its row in flight; NVFP4, whose codes need
+//    the row's maximum first, reads the row a second time while it is still
+//    in L1 or L2, which beat keeping it in registers (occupancy);
 //  * a quotient by an E4M3 scale is a product with its reciprocal and one
 //    correction step (Markstein, "Computation of elementary functions on the
 //    IBM RISC System/6000 processor", 1990): the correctly rounded quotient
@@ -34,9 +34,9 @@ namespace fp4 {
 
 constexpr int kQuantThreads = 256;
 constexpr int kQuantWarps = kQuantThreads / 32;
-// Pieces of 256 values that a warp keeps in registers.
-template <typename T, int FMT>
-constexpr int kKeep = (FMT == kMx ? 8 : 16) / sizeof(T);
+// Pieces of 256 values that a warp has in flight.
+template <typename T>
+constexpr int kAhead = 8 / sizeof(T);
 
 template <typename T>
 __device__ __forceinline__ float to_float(T v) { return static_cast<float>(v); }
@@ -131,7 +131,7 @@ __device__ __forceinline__ float e4m3_value(uint32_t byte) {
 // 256 values from (i * warps_per_row + its place in the row) * 256. Every warp walks
 // the padded extent, so all scale bytes of the row tiles are written.
 template <typename T, int FMT, bool VEC>
-__global__ void __launch_bounds__(kQuantThreads, FMT == kMx ? 4 : 2) quantize_kernel(const QuantParams p, int warps_per_row) {
+__global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantParams p, int warps_per_row) {
   __shared__ uint32_t tops[kQuantWarps];
   grid_launch_dependents();  // a product of these codes may fetch its other operand meanwhile
   const int warp = warp_id(), lane = lane_id();
@@ -145,26 +145,26 @@ __global__ void __launch_bounds__(kQuantThreads, FMT == kMx ? 4 : 2) quantize_ke
   const int64_t row = part * p.rows + r;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const int extent = static_cast<int>(p.groups) * 4 * block_of(FMT);
-  const int step = warps_per_row * 256;
-  const int p0 = place * 256 + blockIdx.y * kKeep<T, FMT> * step;  // first column of the warp (grid.y is 1 in NVFP4)
+  const int step = warps_per_row * 256, stride = kAhead<T> * step;
+  const int p0 = place * 256 + blockIdx.y * stride;  // first column of the warp (grid.y is 1 in NVFP4)
   const int c0 = p0 + lane * 8;
   const int K = live ? p.K : 0;  // rows of the padding hold nothing
 
-  Raw<T> raw[kKeep<T, FMT>];
+  Raw<T> raw[kAhead<T>];
+  auto load_pieces = [&](int c) {
 #pragma unroll
-  for (int i = 0; i < kKeep<T, FMT>; ++i) {
-    raw[i].zero();
-    if (c0 + i * step < K) raw[i].template load<VEC>(x, c0 + i * step, K);
-  }
+    for (int i = 0; i < kAhead<T>; ++i) {
+      raw[i].zero();
+      if (c + i * step < K) raw[i].template load<VEC>(x, c + i * step, K);
+    }
+  };
   float factor = 1.f, inv_factor = 1.f;
   if constexpr (FMT == kNv) {
     uint32_t t = 0;
+    for (int c = c0; c - lane * 8 < K; c += stride) {
+      load_pieces(c);
 #pragma unroll
-    for (int i = 0; i < kKeep<T, FMT>; ++i) t = Raw<T>::max_of(t, raw[i].top());
-    for (int c = c0 + kKeep<T, FMT> * step; c < K; c += step) {
-      Raw<T> v;
-      v.template load<VEC>(x, c, K);
-      t = Raw<T>::max_of(t, v.top());
+      for (int i = 0; i < kAhead<T>; ++i) t = Raw<T>::max_of(t, raw[i].top());
     }
     uint32_t top = __reduce_max_sync(0xffffffffu, Raw<T>::top_bits(t));
     if (warps_per_row > 1) {  // the same for every thread of the CTA
@@ -215,17 +215,14 @@ __global__ void __launch_bounds__(kQuantThreads, FMT == kMx ? 4 : 2) quantize_ke
       if (live && (c >> 1) < p.ldq) *reinterpret_cast<uint32_t*>(q + (c >> 1)) = codes;
     }
   };
+  // (in NVFP4 the row was read just before: its lines are still near)
+  for (int c = p0; c < extent; c += stride) {
+    load_pieces(c + lane * 8);
 #pragma unroll
-  for (int i = 0; i < kKeep<T, FMT>; ++i) {
-    if (p0 + i * step < extent) emit(raw[i], c0 + i * step);  // warp-uniform
-  }
-  if constexpr (FMT == kNv) {
-    for (int c = c0 + kKeep<T, FMT> * step; c - lane * 8 < extent; c += step) {
-      Raw<T> v;
-      v.zero();
-      if (c < K) v.template load<VEC>(x, c, K);
-      emit(v, c);
+    for (int i = 0; i < kAhead<T>; ++i) {
+      if (c + i * step < extent) emit(raw[i], c + i * step + lane * 8);  // warp-uniform
     }
+    if constexpr (FMT == kMx) break;  // the next columns are another CTA's
   }
 }
 
@@ -241,8 +238,8 @@ template <typename T, int FMT>
 cudaError_t quantize_typed(const QuantParams& p, cudaStream_t stream) {
   const bool vec = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.ldx % (16 / sizeof(T)) == 0;
   const int64_t slots = p.parts * ((p.rows + 127) / 128 * 128);
-  const int wpr = row_warps(slots, (p.K + 255) / 256, kKeep<T, FMT>);
-  const int64_t extent = p.groups * 4 * block_of(FMT), share = static_cast<int64_t>(wpr) * kKeep<T, FMT> * 256;
+  const int wpr = row_warps(slots, (p.K + 255) / 256, kAhead<T>);
+  const int64_t extent = p.groups * 4 * block_of(FMT), share = static_cast<int64_t>(wpr) * kAhead<T> * 256;
   const dim3 grid(static_cast<unsigned>((slots * wpr + kQuantWarps - 1) / kQuantWarps),
                   FMT == kMx ? static_cast<unsigned>((extent + share - 1) / share) : 1u);
   if (vec)

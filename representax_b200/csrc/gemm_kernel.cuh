@@ -27,6 +27,7 @@
 // backward; this kernel replaces both.
 #pragma once
 #include "common.h"
+#include "elect.cuh"
 #include "gelu.cuh"
 #include "philox.cuh"
 #include "sm100.cuh"
@@ -727,8 +728,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (even CTA)
-    if (leader && lane == 0) {
+    // The whole warp runs the loop and one lane issues, so that descriptors stay in uniform registers.
+    if (leader) {
       constexpr uint32_t IDESC = idesc_bf16_f32(2 * BM, BN, A_MN, B_MN);
+      const uint64_t a0 = A_MN ? smem_desc_sw128(smem_u32(sA), 8192, 1024) : smem_desc_sw128(smem_u32(sA), 16, 1024);
+      const uint64_t b0 = B_MN ? smem_desc_sw128(smem_u32(sB), 8192, 1024) : smem_desc_sw128(smem_u32(sB), 16, 1024);
+      auto ready = [&](uint64_t* bar, uint32_t parity) -> bool {
+        const bool now = mbar_try_wait(bar, parity) || (*abort_flag == 0 && mbar_wait(bar, parity, p.timeout_ns));
+        return __all_sync(0xffffffffu, now);
+      };
       int stage = 0;
       uint32_t phase = 0;
       int local = 0;
@@ -737,43 +745,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         int m0, n0, kb0, kb1;
         decode(u, m0, n0, kb0, kb1);
         const int acc = local & 1;
-        const uint32_t acc_phase = (local >> 1) & 1;
-        if (*abort_flag || !mbar_wait(&tempty[acc], acc_phase ^ 1, p.timeout_ns)) {
-          report_status(p.status, kStatusTimeoutMma);
-          *abort_flag = 1;
-          break;
-        }
+        ok = ready(&tempty[acc], ((local >> 1) & 1) ^ 1);
+        if (!ok) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (*abort_flag || !mbar_wait(&full[stage], phase, p.timeout_ns)) {
-            report_status(p.status, kStatusTimeoutMma);
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
+          ok = ready(&full[stage], phase);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t a_addr = smem_u32(sA + stage * A_BYTES);
-          const uint32_t b_addr = smem_u32(sB + stage * B_BYTES);
+          const uint64_t a = a0 + static_cast<uint32_t>(stage * (A_BYTES >> 4));
+          const uint64_t b = b0 + static_cast<uint32_t>(stage * (B_BYTES >> 4));
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk) {
-            const uint64_t ad = A_MN ? smem_desc_sw128(a_addr + kk * 2048, 8192, 1024)
-                                     : smem_desc_sw128(a_addr + kk * 32, 16, 1024);
-            const uint64_t bd = B_MN ? smem_desc_sw128(b_addr + kk * 2048, 8192, 1024)
-                                     : smem_desc_sw128(b_addr + kk * 32, 16, 1024);
-            umma_f16_ss_pair(d_tmem, ad, bd, IDESC, (kb > kb0 || kk > 0) ? 1u : 0u);
+            for (int kk = 0; kk < BK / 16; ++kk)
+              umma_f16_ss_pair(d_tmem, a + kk * (A_MN ? 128 : 2), b + kk * (B_MN ? 128 : 2), IDESC,
+                               (kb > kb0 || kk > 0) ? 1u : 0u);
+            umma_commit_pair(&empty[stage], 0x3);
+            if (kb + 1 == kb1) umma_commit_pair(&tfull[acc], 0x3);
           }
-          umma_commit_pair(&empty[stage], 0x3);
+          __syncwarp();
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
           }
         }
-        if (!ok) break;
-        umma_commit_pair(&tfull[acc], 0x3);
+      }
+      if (!ok) {
+        if (lane == 0) report_status(p.status, kStatusTimeoutMma);
+        *abort_flag = 1;
       }
       // Signal both CTAs once every MMA of this pair has retired.
-      umma_commit_pair(drain, 0x3);
+      if (elect_one()) umma_commit_pair(drain, 0x3);
     }
     if (lane == 0 && !mbar_wait(drain, 0, p.timeout_ns)) report_status(p.status, kStatusTimeoutDrain);
     __syncwarp();
