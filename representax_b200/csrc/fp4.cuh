@@ -14,6 +14,8 @@
 // of groups is padded to 256 values of K, the extent of one pipeline stage, so
 // a stage's groups are one contiguous bulk copy.
 #pragma once
+#include <cuda_fp16.h>
+#include <cuda_fp4.h>
 #include <stdint.h>
 
 #include "elect.cuh"
@@ -52,16 +54,27 @@ __device__ __forceinline__ uint32_t pack8(const float (&v)[8]) {
   return out;
 }
 
+// The inverse: eight codes -> their values (exact).
+__device__ __forceinline__ void unpack8(uint32_t codes, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(codes >> (8 * i)), __NV_E2M1);
+    const float2 f = __half22float2(__half2(h));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+
 // MXFP4 scale byte of a block whose largest magnitude has the float bits `top`:
 // e = ceil(log2(top / 6)), at least -126, so that no code saturates (the rule of
-// the MXFP8 quantiser); byte 127 (a factor of one) for a block of zeros; the
-// NaN byte 0xff for a block that holds an infinity or a NaN, so that products
-// with it are NaN.
+// the MXFP8 quantiser). With top = m 2^k, 1 <= m < 2, and 6 = 1.5 * 2^2 that is
+// k - 2 for m <= 1.5 and k - 1 above: no division. Byte 127 (a factor of one) for
+// a block of zeros; the NaN byte 0xff for a block that holds an infinity or a
+// NaN, so that products with it are NaN.
 __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t top) {
   if (top >= 0x7f800000u) return 0xffu;
-  const uint32_t b = __float_as_uint(__fdiv_rn(__uint_as_float(top), 6.f));
-  if (b == 0u) return 127u;
-  return max((b >> 23) + ((b & 0x7fffffu) != 0u ? 1u : 0u), 1u);
+  if (top == 0u) return 127u;
+  return static_cast<uint32_t>(max(static_cast<int>(top >> 23) - 2 + ((top & 0x7fffffu) > 0x400000u ? 1 : 0), 1));
 }
 // 2^-e of a scale byte (1 to 253; 0 for the NaN byte, whose codes do not matter).
 __device__ __forceinline__ float mx_inverse(uint32_t byte) {

@@ -27,6 +27,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "fp4.cuh"
 
 namespace rx {
@@ -58,14 +60,10 @@ struct Raw {
   static constexpr int kWords = 2 * sizeof(T);
   uint32_t w[kWords];
 
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = 0u;
-  }
-  // Columns c.. of a row, zeros past K.
-  template <bool VEC>
+  // Columns c.. of a row: VEC 16-byte loads where all eight exist (always, with FULL), zeros past K.
+  template <bool VEC, bool FULL>
   __device__ __forceinline__ void load(const T* row, int c, int K) {
-    if (VEC && c + 8 <= K) {
+    if (VEC && (FULL || c + 8 <= K)) {
 #pragma unroll
       for (int i = 0; i < kWords / 4; ++i) {
         const uint4 v = ldg_v4_issue(reinterpret_cast<const uint4*>(row + c) + i);
@@ -75,38 +73,40 @@ struct Raw {
         w[4 * i + 3] = v.w;
       }
     } else {
-      zero();
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = 0u;
       T* e = reinterpret_cast<T*>(w);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (c + i < K) e[i] = row[c + i];
     }
   }
-  // Bits of the largest magnitude, comparable as integers (NaN above infinity above finite
-  // values): in each half of the word for 16-bit types.
+  // Largest magnitude, in each half of the word for 16-bit types; a NaN stays one.
   __device__ __forceinline__ uint32_t top() const {
-    uint32_t t = 0;
+    uint32_t t = w[0] & kMagnitude;
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-      if constexpr (sizeof(T) == 2)
-        t = __vmaxu2(t, w[i] & 0x7fff7fffu);
-      else
-        t = max(t, w[i] & 0x7fffffffu);
-    }
+    for (int i = 1; i < kWords; ++i) t = max_of(t, w[i] & kMagnitude);
     return t;
+  }
+  static constexpr uint32_t kMagnitude = sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu;
+  static __device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 4) return max(a, b);  // as integers: NaN above infinity above finite values
+    if constexpr (std::is_same<T, __half>::value) {
+      const __half2 m = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+      return *reinterpret_cast<const uint32_t*>(&m);
+    } else {
+      const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+      return *reinterpret_cast<const uint32_t*>(&m);
+    }
   }
   // Float bits of a magnitude from top().
   static __device__ __forceinline__ uint32_t top_bits(uint32_t t) {
-    if constexpr (sizeof(T) == 4) return t;
-    const uint32_t m = max(t & 0xffffu, t >> 16);
-    if constexpr (sizeof(T) == 2) {
-      const unsigned short h = static_cast<unsigned short>(m);
+    if constexpr (sizeof(T) == 4) {
+      return t;
+    } else {
+      const unsigned short h = static_cast<unsigned short>(max(t & 0xffffu, t >> 16));  // magnitudes order as integers
       return __float_as_uint(to_float(*reinterpret_cast<const T*>(&h))) & 0x7fffffffu;
     }
-    return m;
-  }
-  static __device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b) {
-    return sizeof(T) == 2 ? __vmaxu2(a, b) : max(a, b);
   }
   __device__ __forceinline__ void values(float (&v)[8]) const {
     const T* e = reinterpret_cast<const T*>(w);
@@ -125,6 +125,12 @@ __device__ __forceinline__ float row_factor(uint32_t top) {
 
 __device__ __forceinline__ float e4m3_value(uint32_t byte) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
+}
+
+// a / s correctly rounded, with inv = 1 / s correctly rounded (0 for s = 0): Markstein's correction of a * inv.
+__device__ __forceinline__ float quotient(float a, float s, float inv) {
+  const float guess = a * inv;
+  return fmaf(fmaf(-guess, s, a), inv, guess);
 }
 
 // A row belongs to `warps_per_row` warps (1, 2, 4 or 8); piece i of a warp is the
@@ -147,22 +153,23 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantP
   const int extent = static_cast<int>(p.groups) * 4 * block_of(FMT);
   const int step = warps_per_row * 256, stride = kAhead<T> * step;
   const int p0 = place * 256 + blockIdx.y * stride;  // first column of the warp (grid.y is 1 in NVFP4)
-  const int c0 = p0 + lane * 8;
   const int K = live ? p.K : 0;  // rows of the padding hold nothing
 
   Raw<T> raw[kAhead<T>];
-  auto load_pieces = [&](int c) {
+  auto load_pieces = [&](int c, bool full) {  // c: the warp's first column
 #pragma unroll
     for (int i = 0; i < kAhead<T>; ++i) {
-      raw[i].zero();
-      if (c + i * step < K) raw[i].template load<VEC>(x, c + i * step, K);
+      if (full)
+        raw[i].template load<VEC, true>(x, c + lane * 8 + i * step, K);
+      else
+        raw[i].template load<VEC, false>(x, c + lane * 8 + i * step, K);
     }
   };
   float factor = 1.f, inv_factor = 1.f;
   if constexpr (FMT == kNv) {
     uint32_t t = 0;
-    for (int c = c0; c - lane * 8 < K; c += stride) {
-      load_pieces(c);
+    for (int c = p0; c < K; c += stride) {
+      load_pieces(c, c + (kAhead<T> - 1) * step + 256 <= K);
 #pragma unroll
       for (int i = 0; i < kAhead<T>; ++i) t = Raw<T>::max_of(t, raw[i].top());
     }
@@ -181,7 +188,7 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantP
   const int64_t sf_row = part * padded + r;
   uint8_t* sf = p.sf + scale_offset(sf_row, 0, p.groups);
   uint8_t* q = p.q + row * p.ldq;
-  auto emit = [&](const Raw<T>& in, int c) {
+  auto emit = [&](const Raw<T>& in, int c, bool full) {
     uint32_t t = in.top(), byte;
     float v[8];
     in.values(v);
@@ -193,15 +200,12 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantP
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] *= inv;
     } else {
-      const float want = __fdiv_rn(__uint_as_float(Raw<T>::top_bits(t)), 6.f) * inv_factor;
+      const float want = quotient(__uint_as_float(Raw<T>::top_bits(t)) * inv_factor, 6.f, 1.f / 6.f);
       byte = __nv_cvt_float_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
       // a row with a NaN factor is NaN by that factor whatever its codes; a zero scale has zero codes
       const float s = e4m3_value(byte), inv = s > 0.f ? __frcp_rn(s) : 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float a = v[i] * inv_factor, guess = a * inv;
-        v[i] = fmaf(fmaf(-guess, s, a), inv, guess);
-      }
+      for (int i = 0; i < 8; ++i) v[i] = quotient(v[i] * inv_factor, s, inv);
     }
     const uint32_t codes = pack8(v);
     // four blocks' bytes -> one 4-byte word of the group, written by its first lane
@@ -209,18 +213,30 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantP
     uint32_t word = byte << (8 * ((lane / kLanes) & 3));
 #pragma unroll
     for (int o = kLanes; o < 4 * kLanes; o *= 2) word |= __shfl_xor_sync(0xffffffffu, word, o);
-    if (c < extent) {
-      if (lane % (4 * kLanes) == 0)
-        *reinterpret_cast<uint32_t*>(sf + static_cast<int64_t>(c / (4 * block_of(FMT))) * 512) = live ? word : 0u;
+    if (full) {
+      if (lane % (4 * kLanes) == 0) *reinterpret_cast<uint32_t*>(sf + static_cast<int64_t>(c / (4 * block_of(FMT))) * 512) = word;
+      *reinterpret_cast<uint32_t*>(q + (c >> 1)) = codes;
+    } else if (c < extent) {
+      if (lane % (4 * kLanes) == 0) *reinterpret_cast<uint32_t*>(sf + static_cast<int64_t>(c / (4 * block_of(FMT))) * 512) = live ? word : 0u;
       if (live && (c >> 1) < p.ldq) *reinterpret_cast<uint32_t*>(q + (c >> 1)) = codes;
     }
   };
   // (in NVFP4 the row was read just before: its lines are still near)
   for (int c = p0; c < extent; c += stride) {
-    load_pieces(c + lane * 8);
+    const bool full = c + (kAhead<T> - 1) * step + 256 <= K;  // warp-uniform: no bounds inside
+    load_pieces(c, full);
+    if (full) {
 #pragma unroll
-    for (int i = 0; i < kAhead<T>; ++i) {
-      if (c + i * step < extent) emit(raw[i], c + i * step + lane * 8);  // warp-uniform
+      for (int i = 0; i < kAhead<T>; ++i) emit(raw[i], c + i * step + lane * 8, true);
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < kAhead<T>; ++i) {
+        Raw<T> in = raw[0];
+#pragma unroll
+        for (int j = 1; j < kAhead<T>; ++j)
+          if (j == i) in = raw[j];
+        if (c + i * step < extent) emit(in, c + i * step + lane * 8, false);
+      }
     }
     if constexpr (FMT == kMx) break;  // the next columns are another CTA's
   }
@@ -281,15 +297,11 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const Dequant
       scale = byte == 0xffu ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
     else
       scale = e4m3_value(byte) * factor;
+    float f[8];
+    unpack8(codes, f);
     T v[kVals];
 #pragma unroll
-    for (int j = 0; j < kVals; ++j) {
-      const uint32_t n = (codes >> (4 * j)) & 0xfu;
-      // magnitude codes 0..7: 0, 0.5, then (1 + m / 2) 2^(e - 1)
-      const uint32_t mag = n & 7u;
-      const float m = mag < 2u ? 0.5f * mag : __uint_as_float(((mag >> 1) + 126u) << 23 | (mag & 1u) << 22);
-      v[j] = from_float<T>((n & 8u ? -m : m) * scale);
-    }
+    for (int j = 0; j < kVals; ++j) v[j] = from_float<T>(f[j] * scale);
     if (vec && c + kVals <= p.K) {
       *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<const uint4*>(v);
     } else {

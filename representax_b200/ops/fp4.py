@@ -251,7 +251,11 @@ def quantize_reference(x: torch.Tensor, fmt: str) -> tuple[torch.Tensor, torch.T
     row = None
     nan = torch.full((), float("nan"), device=x.device)
     if fmt == "mxfp4":
-        scale = torch.where(amax.isfinite(), _pow2_ceil(amax / six), nan)
+        # ceil(log2(amax / 6)) from amax = m 2^e, 0.5 <= m < 1: e - 3 for m <= 0.75, e - 2 above
+        mantissa, exponent = torch.frexp(amax)
+        e = torch.where(mantissa <= 0.75, exponent - 3, exponent - 2).clamp(min=-126)
+        scale = torch.where(amax > 0, torch.ldexp(torch.ones_like(amax), e), torch.ones_like(amax))
+        scale = torch.where(amax.isfinite(), scale, nan)
         full = scale
     else:
         top = amax.amax(1) if amax.shape[1] else amax.sum(1)
