@@ -138,6 +138,13 @@ std::vector<at::Tensor> gated_ffn_backward(const at::Tensor& dy, const c10::opti
                                            const c10::optional<at::Tensor>& exps, const std::vector<bool>& need,
                                            const std::vector<c10::optional<at::Tensor>>& acc,
                                            const std::vector<at::ScalarType>& like, const at::Tensor& status);
+at::Tensor gated_ffn_apply(const at::Tensor& x, const at::Tensor& gate_up, const at::Tensor& down,
+                           const c10::optional<at::Tensor>& gate_up_bias, const c10::optional<at::Tensor>& down_bias,
+                           const c10::optional<at::Tensor>& residual, int64_t act, const at::Tensor& status);
+at::Tensor fp4_linear_apply(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_sf,
+                            const c10::optional<at::Tensor>& w_row, int64_t parts, int64_t fmt,
+                            const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual,
+                            const at::Tensor& status);
 std::vector<at::Tensor> fp4_quantize(const at::Tensor& x, int64_t parts, int64_t fmt);
 void fp4_dequantize(const at::Tensor& q, const at::Tensor& sf, const c10::optional<at::Tensor>& row_scale, int64_t parts,
                     int64_t fmt, at::Tensor& out);
@@ -234,6 +241,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fp4_dequantize", &rx::fp4_dequantize, "values of MXFP4 / NVFP4 codes and scales");
   m.def("gated_ffn_forward", &rx::gated_ffn_forward, "forward of the gated feed-forward block");
   m.def("gated_ffn_backward", &rx::gated_ffn_backward, "gradients of the gated feed-forward block");
+  m.def("gated_ffn_apply", &rx::gated_ffn_apply, "the gated feed-forward block as an autograd node (bf16 parameters)");
+  m.def("fp4_linear_apply", &rx::fp4_linear_apply, "the 4-bit linear layer as an autograd node");
   m.def("fp4_gemm", &rx::fp4_gemm, "tcgen05 block-scaled 4-bit GEMM");
   m.def("fp4_linear", &rx::fp4_linear, "linear layer: activations quantised to 4 bits, 4-bit weight");
   m.def("fp4_linear_dgrad", &rx::fp4_linear_dgrad, "input gradient of the 4-bit linear layer");

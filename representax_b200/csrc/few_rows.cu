@@ -1,14 +1,12 @@
-// y = x W^T for few token rows (1 to 64): a single query's tokens through a
-// layer, in bf16 or with both operands in microscaled 4 bits, plain
+// y = x W^T for few token rows: a single query's tokens through a layer, in bf16 or with both operands in microscaled 4 bits, plain
 // (+ bias + residual) or as the gated projection act(x Wg^T) * (x Wu^T).
 //
 // The work is reading W once, so everything serves memory parallelism. The
 // roles of the operands are swapped: 128 weight rows are the M side of the
-// tensor core's tile and the T tokens (padded to 16, 32 or 64) its N side, so no
-// product is spent on 128-row padding of T and the output columns give many
-// tiles. K is split over the CTAs of a cluster until the grid fills the GPU
-// twice over; each CTA streams its share of W through a TMA ring (about 100 KB,
-// two CTAs per SM) into fp32 TMEM accumulators. The partial sums meet in
+// tensor core's tile and the T tokens (in tiles of 16, 32, 64 or 128) its N side,
+// so little is spent on padding of T and the output columns give many tiles. K is split over the CTAs of a cluster until the grid fills the GPU
+// twice over; each CTA streams its share of W through a TMA ring
+// (two or three CTAs per SM) into fp32 TMEM accumulators. The partial sums meet in
 // shared memory: after a cluster barrier every warp of the cluster takes
 // a token's 128 outputs, adds the partials of all CTAs, read through
 // distributed shared memory, in rank order (so results do not depend on timing)
@@ -37,7 +35,6 @@ namespace few {
 constexpr int kThreads = 192;  // producer, MMA issuer, four TMEM readers
 constexpr int kWarps = kThreads / 32;
 constexpr int kTileW = 128 * 128;  // 128 weight rows x 128 bytes
-constexpr int kRingBytes = 100 * 1024;
 constexpr int kPartLd = 132;       // floats per token row of the partial sums
 
 template <int KIND, int PARTS, int NT>
@@ -46,7 +43,12 @@ struct Shape {
   static constexpr int kSfW = PARTS * kGroups * 512, kSfX = kGroups * 512;
   static constexpr int kTiles = PARTS * kTileW + NT * 128;
   static constexpr int kStage = kTiles + (kSfW + kSfX + 1023) / 1024 * 1024;
-  static constexpr int kStages = kRingBytes / kStage;
+  // Ring: enough bytes in flight to cover the latency, little enough that three CTAs fit an SM. At one token
+  // (K 2048, 12288 outputs, NVFP4) 104 KB took 9.0 us and 72 KB 6.6 us; the plain bf16 stream, which starts
+  // under the gated kernel's tail, gained from 90 KB (block of one token 20.3 -> 19.5 us), 128-token tiles from a
+  // third stage (128 tokens, K 6144: 18.6 -> 16.8 us).
+  static constexpr int kRingBytes = (NT == 128 ? 104 : (KIND == kBf16 && PARTS == 1 ? 90 : 72)) * 1024;
+  static constexpr int kStages = kRingBytes / kStage < 2 ? 2 : kRingBytes / kStage;
   static constexpr int kPart = PARTS * NT * kPartLd * 4;
   static constexpr int kData = kStages * kStage > kPart ? kStages * kStage : kPart;
   static constexpr int kSmem = 1024 + kData + 256;
@@ -54,7 +56,7 @@ struct Shape {
   static constexpr int kAccCols = (PARTS - 1) * NT + (NT < 32 ? 32 : NT);
   static constexpr int kCols = kAccCols + (PARTS + 1) * kGroups * 4;
   static constexpr int kTmemCols = kCols <= 32 ? 32 : (kCols <= 64 ? 64 : (kCols <= 128 ? 128 : 256));
-  static_assert(kStages >= 2 && kCols <= 256, "two CTAs per SM must fit");
+  static_assert(kCols <= 256 && 2 * kSmem <= 220 * 1024, "two CTAs per SM must fit");
 };
 
 // Four consecutive floats of another CTA's shared memory.
@@ -78,7 +80,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int warp = warp_id(), lane = lane_id();
   const int rank = static_cast<int>(cluster_ctarank());
   const int splits = static_cast<int>(gridDim.y);  // the cluster spans the whole y dimension
-  const int tile = blockIdx.x;
+  const int tile = blockIdx.x, t0 = blockIdx.z * NT;  // weight rows (output columns), first token
+  const int tokens = min(NT, p.T - t0);
   const int kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * rank / splits);
   const int kb1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (rank + 1) / splits);
 
@@ -99,9 +102,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   };
   auto load_x = [&](int kb, int s) {
     uint8_t* dst = base + s * S::kStage;
-    tma_load_2d(dst + PARTS * kTileW, &tmX, &full[s], kb * (KIND == kBf16 ? 64 : 128), 0);
+    tma_load_2d(dst + PARTS * kTileW, &tmX, &full[s], kb * (KIND == kBf16 ? 64 : 128), t0);
     if constexpr (KIND != kBf16)
-      bulk_load(dst + S::kTiles + S::kSfW, p.sf_x + static_cast<int64_t>(kb) * S::kGroups * 512, S::kSfX, &full[s]);
+      bulk_load(dst + S::kTiles + S::kSfW, p.sf_x + ((t0 >> 7) * p.groups + static_cast<int64_t>(kb) * S::kGroups) * 512,
+                S::kSfX, &full[s]);
   };
 
   const int first = min(S::kStages, kb1 - kb0);  // K blocks that fill the empty ring
@@ -227,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         tmem_ld_wait();
 #pragma unroll
         for (int t = 0; t < (NT < 32 ? NT : 32); ++t)
-          if (c * 32 + t < p.T)
+          if (c * 32 + t < tokens)
             part[(b * NT + c * 32 + t) * kPartLd + quad * 32 + lane] = __uint_as_float(r[t]);
       }
     }
@@ -240,14 +244,28 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t part_addr = smem_u32(part) + lane * 16;
   const int n = tile * 128 + lane * 4;
   if (*abort_flag == 0) {
-    for (int t = rank * kWarps + warp; t < p.T; t += splits * kWarps) {
+    for (int tl = rank * kWarps + warp; tl < tokens; tl += splits * kWarps) {
+      const int64_t t = t0 + tl;
+      // what the epilogue reads from memory first, then the partial sums of all CTAs
+      float factor[PARTS][4], bias[PARTS][4], add[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool live = n + j < p.N;
+#pragma unroll
+        for (int b = 0; b < PARTS; ++b) {
+          const int64_t c = static_cast<int64_t>(b) * p.N + n + j;
+          factor[b][j] = KIND == kNvfp4 && live ? p.row_x[t] * p.row_w[c] : 1.f;
+          bias[b][j] = live && p.bias != nullptr ? __bfloat162float(p.bias[c]) : 0.f;
+        }
+        add[j] = PARTS == 1 && live && p.residual != nullptr ? __bfloat162float(p.residual[t * p.ld_res + n + j]) : 0.f;
+      }
       float4 in[PARTS][8];
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         if (r < splits) {
           const uint32_t peer = mapa_shared(part_addr, static_cast<uint32_t>(r));
 #pragma unroll
-          for (int b = 0; b < PARTS; ++b) in[b][r] = ld_cluster_f4(peer + (b * NT + t) * kPartLd * 4);
+          for (int b = 0; b < PARTS; ++b) in[b][r] = ld_cluster_f4(peer + (b * NT + tl) * kPartLd * 4);
         }
       }
       float v[PARTS][4];
@@ -263,23 +281,12 @@ __global__ void __launch_bounds__(kThreads, 2)
             v[b][3] += in[b][r].w;
           }
         }
-        const int64_t c0 = static_cast<int64_t>(b) * p.N + n;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (n + j < p.N) {
-            if constexpr (KIND == kNvfp4) v[b][j] *= p.row_x[t] * p.row_w[c0 + j];
-            if (p.bias != nullptr) v[b][j] += __bfloat162float(p.bias[c0 + j]);
-          }
-        }
+        for (int j = 0; j < 4; ++j) v[b][j] = v[b][j] * factor[b][j] + bias[b][j];
       }
       float y[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        y[j] = v[0][j];
-        if constexpr (PARTS == 2) y[j] = v[1][j];
-        if constexpr (PARTS == 1)
-          if (n + j < p.N && p.residual != nullptr) y[j] += __bfloat162float(p.residual[t * p.ld_res + n + j]);
-      }
+      for (int j = 0; j < 4; ++j) y[j] = PARTS == 2 ? v[1 % PARTS][j] : v[0][j] + add[j];
       if constexpr (PARTS == 2) gated::gate(p.act, v[0], y);
       if constexpr (PARTS == 2 && KIND == kMxfp4) {
         if (p.q_out != nullptr) {  // eight lanes hold a block of 32
@@ -332,10 +339,10 @@ cudaError_t launch_shape(const CUtensorMap& map_x, const CUtensorMap& map_w, con
     if (device >= 0 && device < 64) configured[device] = true;
   }
   // as many K splits as two CTAs per SM can hold at once, each with at least two stages of work
-  const int tiles = (p.N + 127) / 128;
-  const int splits = std::max(1, std::min({8, 2 * sms / tiles, p.k_blocks / 2}));
+  const int tiles = (p.N + 127) / 128, token_tiles = (p.T + NT - 1) / NT;
+  const int splits = std::max(1, std::min({8, 2 * sms / (tiles * token_tiles), p.k_blocks / 2}));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles, splits);
+  cfg.gridDim = dim3(tiles, splits, token_tiles);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = stream;
@@ -357,7 +364,10 @@ cudaError_t launch_parts(const CUtensorMap& mx, const CUtensorMap& mw, const Par
   switch (tile_rows(p.T)) {
     case 16: return launch_shape<KIND, PARTS, 16>(mx, mw, p, sms, device, stream);
     case 32: return launch_shape<KIND, PARTS, 32>(mx, mw, p, sms, device, stream);
-    default: return launch_shape<KIND, PARTS, 64>(mx, mw, p, sms, device, stream);
+    case 64: return launch_shape<KIND, PARTS, 64>(mx, mw, p, sms, device, stream);
+    default:
+      if constexpr (PARTS == 1) return launch_shape<KIND, PARTS, 128>(mx, mw, p, sms, device, stream);
+      return cudaErrorInvalidValue;  // the hosts send gated products of more rows to the GEMM
   }
 }
 

@@ -8,7 +8,15 @@
 namespace rx {
 namespace few {
 
-constexpr int kMaxRows = 64;
+constexpr int64_t kFewTiles = 12;
+
+// Which products run here rather than on the GEMMs' CTA pairs with their 256-row tiles. Plain: where such
+// tiles would leave most of the GPU idle, that is few of them (a pair's 256 x 256 tiles of `rows` x `cols`; 74
+// pairs make a wave), or very few rows. Gated: up to 32 rows (two accumulators leave a ring too short beyond).
+inline bool takes(int64_t rows, int64_t cols, bool gated) {
+  if (gated) return rows <= 32;
+  return rows <= 16 || (rows + 255) / 256 * ((cols + 255) / 256) <= kFewTiles;
+}
 
 enum Kind : int { kBf16 = 0, kMxfp4 = 1, kNvfp4 = 2 };
 
@@ -41,8 +49,8 @@ struct Params {
   uint64_t timeout_ns;
 };
 
-// Rows of a token tile for T token rows (16, 32 or 64).
-inline int tile_rows(int64_t t) { return t <= 16 ? 16 : (t <= 32 ? 32 : 64); }
+// Rows of a token tile for T token rows.
+inline int tile_rows(int64_t t) { return t <= 16 ? 16 : (t <= 32 ? 32 : (t <= 64 ? 64 : 128)); }
 
 // `map_x`: boxes of tile_rows(T) rows x 128 bytes; `map_w`: boxes of 128 rows x 128 bytes.
 cudaError_t launch(int kind, const CUtensorMap& map_x, const CUtensorMap& map_w, const Params& p, int sms, int device,

@@ -124,7 +124,7 @@ at::Tensor bias_gradient(const at::Tensor& dy, const OptTensor& acc, at::ScalarT
 
 }  // namespace
 
-// bf16 products of 1 to 64 token rows x [T, K] with w [parts * N, K]: parts 1: x w^T (+ bias) (+ residual);
+// bf16 products of few token rows x [T, K] with w [parts * N, K]: parts 1: x w^T (+ bias) (+ residual);
 // parts 2 (gate, up): act(x wg^T + bg) * (x wu^T + bu). `after_producer`: the launch just before, one of this kind, wrote x.
 void few_rows_linear(const at::Tensor& x, const at::Tensor& w, int64_t parts, int64_t act,
                      const OptTensor& bias, const OptTensor& residual, at::Tensor& out,
@@ -134,7 +134,7 @@ void few_rows_linear(const at::Tensor& x, const at::Tensor& w, int64_t parts, in
   RX_CHECK(x.dim() == 2 && w.dim() == 2 && w.size(0) % parts == 0, "x and w must be matrices, w of whole parts");
   const int64_t T = x.size(0), K = x.size(1), N = w.size(0) / parts;
   const int dev = x.get_device();
-  RX_CHECK(T >= 1 && T <= few::kMaxRows, "few_rows_linear takes 1 to ", few::kMaxRows, " rows, got ", T);
+  RX_CHECK(T >= 1 && T < (1ll << 20) && (parts == 1 || T <= 64), "few_rows_linear: too many rows, ", T);
   RX_CHECK(K >= 1 && N >= 1 && K < (1ll << 30) && N < (1ll << 29), "bad sizes");
   check_plain(x, "x", T, K, dev);
   check_plain(w, "w", parts * N, K, dev);
@@ -249,24 +249,27 @@ std::vector<at::Tensor> gated_ffn_forward(const at::Tensor& x_in, const at::Tens
   check_bf16(gate_up_in, "gate_up");
   check_bf16(down_in, "down");
   RX_CHECK(x_in.dim() == 2 && gate_up_in.dim() == 2 && down_in.dim() == 2, "x, gate_up and down must be matrices");
-  c10::cuda::CUDAGuard guard(x_in.get_device());
+  const int dev = x_in.get_device();
+  for (const OptTensor& t : {OptTensor(gate_up_in), OptTensor(down_in), gate_up_bias, down_bias, residual_in})
+    RX_CHECK(!t.has_value() || (t->is_cuda() && t->get_device() == dev), "every operand must be on device ", dev, " of x");
+  c10::cuda::CUDAGuard guard(dev);
   const at::Tensor x = rows16(x_in), gate_up = rows16(gate_up_in), down = rows16(down_in);
   const OptTensor b1 = vector16(gate_up_bias), b2 = vector16(down_bias);
   const OptTensor residual = residual_in.has_value() ? OptTensor(rows16(*residual_in)) : residual_in;
   const int64_t T = x.size(0), I = down.size(1), H = down.size(0);
   at::Tensor h = at::empty({T, I}, x.options()), y = at::empty({T, H}, x.options()), saved, exps;
-  const bool few = T <= few::kMaxRows;
+  const bool few_gated = !save && few::takes(T, I, true), few_down = few::takes(T, H, false);
   if (save) {
     saved = at::empty({saved_tiles(T, I), 2, 32, 32}, x.options().dtype(at::kHalf));
     exps = at::empty({saved_tiles(T, I), 32}, x.options().dtype(at::kShort));
     gated_forward(x, gate_up, b1, h, saved, exps, act, status);
-  } else if (few) {
+  } else if (few_gated) {
     few_rows_linear(x, gate_up, 2, act, b1, c10::nullopt, h, false, status);
   } else {
     gated_forward(x, gate_up, b1, h, c10::nullopt, c10::nullopt, act, status);
   }
-  if (few)
-    few_rows_linear(h, down, 1, 0, b2, residual, y, !save, status);
+  if (few_down)
+    few_rows_linear(h, down, 1, 0, b2, residual, y, few_gated, status);
   else
     gemm_tcgen05(h, down, y, false, false, (b2.has_value() ? kBias : 0) | (residual.has_value() ? kResidual : 0), kOutBf16,
                  1.0, b2, c10::nullopt, c10::nullopt, residual, status, 0, 0, 0, 0, 0.0, c10::nullopt);

@@ -50,7 +50,7 @@ struct Operand {
 
 void check_sizes(int64_t rows, int64_t parts, int64_t K) {
   RX_CHECK(parts >= 1 && rows >= 0 && K > 0, "bad sizes");
-  RX_CHECK(K < (1ll << 30) && (rows + 127) / 128 * 128 * parts < (1ll << 30), "matrix too large");
+  RX_CHECK(K < (1ll << 24) && (rows + 127) / 128 * 128 * parts < (1ll << 30), "matrix too large");
 }
 
 // The operand that codes, scales and row factors hold, checked.
@@ -230,7 +230,7 @@ void run_product(const Operand& a, const Operand& b, int64_t act, const OptTenso
     p.timeout_ns = kWaitBudgetNs;
   };
   const CUtensorMap tb = make_tmap_2d_u8(b.q, b.all_rows(), b.code_bytes(), b.ldq, 128);
-  if (M <= few::kMaxRows) {
+  if (few::takes(M, N, b.parts == 2)) {
     const CUtensorMap ta = make_tmap_2d_u8(a.q, M, a.code_bytes(), a.ldq, few::tile_rows(M));
     few::Params p{};
     fill(p);

@@ -133,9 +133,9 @@ __device__ __forceinline__ float quotient(float a, float s, float inv) {
   return fmaf(fmaf(-guess, s, a), inv, guess);
 }
 
-// A row belongs to `warps_per_row` warps (1, 2, 4 or 8); piece i of a warp is the
-// 256 values from (i * warps_per_row + its place in the row) * 256. Every warp walks
-// the padded extent, so all scale bytes of the row tiles are written.
+// A row belongs to `warps_per_row` warps (1, 2, 4 or 8), which take spans of kAhead pieces in turn; in MXFP4,
+// where spans do not depend on one another, blockIdx.y goes over them instead. All scale bytes of the row
+// tiles are written, those of the padding included.
 template <typename T, int FMT, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantParams p, int warps_per_row) {
   __shared__ uint32_t tops[kQuantWarps];
@@ -151,8 +151,9 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantP
   const int64_t row = part * p.rows + r;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const int extent = static_cast<int>(p.groups) * 4 * block_of(FMT);
-  const int step = warps_per_row * 256, stride = kAhead<T> * step;
-  const int p0 = place * 256 + blockIdx.y * stride;  // first column of the warp (grid.y is 1 in NVFP4)
+  constexpr int kSpan = kAhead<T> * 256;                               // consecutive columns that a warp takes at a time
+  const int p0 = (place + blockIdx.y * warps_per_row) * kSpan;        // its first (grid.y is 1 in NVFP4)
+  const int stride = warps_per_row * kSpan;
   const int K = live ? p.K : 0;  // rows of the padding hold nothing
 
   Raw<T> raw[kAhead<T>];
@@ -160,16 +161,16 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantP
 #pragma unroll
     for (int i = 0; i < kAhead<T>; ++i) {
       if (full)
-        raw[i].template load<VEC, true>(x, c + lane * 8 + i * step, K);
+        raw[i].template load<VEC, true>(x, c + lane * 8 + i * 256, K);
       else
-        raw[i].template load<VEC, false>(x, c + lane * 8 + i * step, K);
+        raw[i].template load<VEC, false>(x, c + lane * 8 + i * 256, K);
     }
   };
   float factor = 1.f, inv_factor = 1.f;
   if constexpr (FMT == kNv) {
     uint32_t t = 0;
     for (int c = p0; c < K; c += stride) {
-      load_pieces(c, c + (kAhead<T> - 1) * step + 256 <= K);
+      load_pieces(c, c + kSpan <= K);
 #pragma unroll
       for (int i = 0; i < kAhead<T>; ++i) t = Raw<T>::max_of(t, raw[i].top());
     }
@@ -223,11 +224,11 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantP
   };
   // (in NVFP4 the row was read just before: its lines are still near)
   for (int c = p0; c < extent; c += stride) {
-    const bool full = c + (kAhead<T> - 1) * step + 256 <= K;  // warp-uniform: no bounds inside
+    const bool full = c + kSpan <= K;  // warp-uniform: no bounds inside
     load_pieces(c, full);
     if (full) {
 #pragma unroll
-      for (int i = 0; i < kAhead<T>; ++i) emit(raw[i], c + i * step + lane * 8, true);
+      for (int i = 0; i < kAhead<T>; ++i) emit(raw[i], c + i * 256 + lane * 8, true);
     } else {
 #pragma unroll 1
       for (int i = 0; i < kAhead<T>; ++i) {
@@ -235,18 +236,17 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantP
 #pragma unroll
         for (int j = 1; j < kAhead<T>; ++j)
           if (j == i) in = raw[j];
-        if (c + i * step < extent) emit(in, c + i * step + lane * 8, false);
+        if (c + i * 256 < extent) emit(in, c + i * 256 + lane * 8, false);
       }
     }
     if constexpr (FMT == kMx) break;  // the next columns are another CTA's
   }
 }
 
-// Warps of a row: enough that a warp keeps its whole share in registers, more while the rows are too few to
-// give every SM 16 warps.
-static int row_warps(int64_t slots, int64_t pieces, int keep) {
+// Warps of a row whose `spans` they share: more than one only while the rows are too few to give every SM 16 warps.
+static int row_warps(int64_t rows, int64_t spans) {
   int wpr = 1;
-  while (wpr < kQuantWarps && (pieces > static_cast<int64_t>(wpr) * keep || (wpr < pieces && slots * wpr < 148 * 16))) wpr *= 2;
+  while (wpr < kQuantWarps && wpr < spans && rows * wpr < 148 * 16) wpr *= 2;
   return wpr;
 }
 
@@ -254,10 +254,10 @@ template <typename T, int FMT>
 cudaError_t quantize_typed(const QuantParams& p, cudaStream_t stream) {
   const bool vec = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.ldx % (16 / sizeof(T)) == 0;
   const int64_t slots = p.parts * ((p.rows + 127) / 128 * 128);
-  const int wpr = row_warps(slots, (p.K + 255) / 256, kAhead<T>);
-  const int64_t extent = p.groups * 4 * block_of(FMT), share = static_cast<int64_t>(wpr) * kAhead<T> * 256;
+  const int64_t extent = p.groups * 4 * block_of(FMT), spans = (extent + kAhead<T> * 256 - 1) / (kAhead<T> * 256);
+  const int wpr = FMT == kMx ? 1 : row_warps(slots, spans);
   const dim3 grid(static_cast<unsigned>((slots * wpr + kQuantWarps - 1) / kQuantWarps),
-                  FMT == kMx ? static_cast<unsigned>((extent + share - 1) / share) : 1u);
+                  FMT == kMx ? static_cast<unsigned>(spans) : 1u);
   if (vec)
     quantize_kernel<T, FMT, true><<<grid, kQuantThreads, 0, stream>>>(p, wpr);
   else
@@ -316,7 +316,7 @@ template <typename T>
 cudaError_t dequantize_typed(const DequantParams& p, int fmt, cudaStream_t stream) {
   const bool vec = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo % (16 / sizeof(T)) == 0;
   const int64_t rows = p.parts * p.rows;
-  const int wpr = row_warps(rows, (p.K + 512 / static_cast<int>(sizeof(T)) - 1) / (512 / static_cast<int>(sizeof(T))), 16);
+  const int wpr = row_warps(rows, p.K / (512 / static_cast<int>(sizeof(T))));
   const unsigned grid = static_cast<unsigned>((rows * wpr + kQuantWarps - 1) / kQuantWarps);
   if (fmt == kMx)
     dequantize_kernel<T, kMx><<<grid, kQuantThreads, 0, stream>>>(p, wpr, vec);

@@ -36,24 +36,28 @@ def _check(x, gate_up, down, activation, gate_up_bias, down_bias, residual) -> N
         raise ValueError(f"unsupported activation {activation!r}")
     if x.dim() != 2 or gate_up.dim() != 2 or down.dim() != 2:
         raise ValueError("x, gate_up and down must be matrices")
-    width = down.shape[1]
-    if tuple(gate_up.shape) != (2 * width, x.shape[1]) or down.shape[0] != x.shape[1]:
+    hidden, width = down.shape
+    if x.shape[1] != hidden or gate_up.shape != (2 * width, hidden):
         raise ValueError(f"gate_up must be [2 I, H] and down [H, I] for x [T, H]: got {tuple(gate_up.shape)}, "
                          f"{tuple(down.shape)} and {tuple(x.shape)}")
-    if gate_up_bias is not None and tuple(gate_up_bias.shape) != (2 * width,):
+    if gate_up_bias is not None and gate_up_bias.shape != (2 * width,):
         raise ValueError(f"gate_up_bias must be [{2 * width}]")
-    if down_bias is not None and tuple(down_bias.shape) != (down.shape[0],):
-        raise ValueError(f"down_bias must be [{down.shape[0]}]")
+    if down_bias is not None and down_bias.shape != (hidden,):
+        raise ValueError(f"down_bias must be [{hidden}]")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError("residual must have the shape and type of x")
-    for name, t in (("gate_up", gate_up), ("down", down), ("gate_up_bias", gate_up_bias), ("down_bias", down_bias),
-                    ("residual", residual)):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
 
 
-def _view(param):
-    return None if param is None else compute_view(param)
+def plain(param) -> bool:
+    """A bf16 tensor with nothing attached (compute copy, fp32 accumulator, shards): its own compute copy."""
+
+    return param is None or (param.dtype is torch.bfloat16 and not param.__dict__)
+
+
+def view(param):
+    """The bf16 compute copy of a parameter, or None."""
+
+    return param if plain(param) else computeview(param)
 
 
 class GatedFeedForwardFn(torch.autograd.Function):
@@ -61,7 +65,7 @@ class GatedFeedForwardFn(torch.autograd.Function):
     def forward(ctx, x, gate_up, down, gate_up_bias, down_bias, residual, act):
         need = ctx.needs_input_grad
         through_z = need[0] or need[1] or need[3]
-        y, h, saved, exps = ext().gated_ffn_forward(x, _view(gate_up), _view(down), _view(gate_up_bias), _view(down_bias),
+        y, h, saved, exps = ext().gated_ffn_forward(x, view(gate_up), view(down), view(gate_up_bias), view(down_bias),
                                                     residual, act, through_z, status(x.device))
         # kept only as far as the gradients asked for need it
         ctx.save_for_backward(x if need[1] else None, gate_up, down, gate_up_bias, down_bias, h if need[2] else None, saved,
@@ -75,7 +79,7 @@ class GatedFeedForwardFn(torch.autograd.Function):
         params = (None, gate_up, down, b1, b2)
         acc = [None if p is None else getattr(p, "main_grad", None) for p in params]
         like = [dy.dtype if p is None else p.dtype for p in params]
-        grads = ext().gated_ffn_backward(dy, x, h, _view(gate_up), _view(down), saved, exps, need, acc, like,
+        grads = ext().gated_ffn_backward(dy, x, h, view(gate_up), view(down), saved, exps, need, acc, like,
                                          status(dy.device))
         return (*grads, dy if ctx.needs_input_grad[5] else None, None)
 
@@ -107,8 +111,10 @@ def gated_feed_forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tenso
         args = (x, gate_up, down, gate_up_bias, down_bias, residual)
         act = _codes()[activation]
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+            if plain(gate_up) and plain(down) and plain(gate_up_bias) and plain(down_bias):
+                return ext().gated_ffn_apply(*args, act, status(x.device))
             return GatedFeedForwardFn.apply(*args, act)
-        return ext().gated_ffn_forward(x, _view(gate_up), _view(down), _view(gate_up_bias), _view(down_bias), residual, act,
+        return ext().gated_ffn_forward(x, view(gate_up), view(down), view(gate_up_bias), view(down_bias), residual, act,
                                        False, status(x.device))[0]
     return gated_feed_forward_reference(x, gate_up, down, activation, gate_up_bias, down_bias, residual)
 

@@ -31,7 +31,8 @@ from dataclasses import dataclass
 import torch
 
 from ._ext import ext, status
-from .functional import _colsum_into, _GradSink, compute_view
+from .ffn import plain, view
+from .functional import _colsum_into, _GradSink
 
 FORMATS = {"mxfp4": 1, "nvfp4": 2}
 BLOCK = {"mxfp4": 32, "nvfp4": 16}
@@ -123,9 +124,9 @@ def dequantize(op: FP4Operand, dtype: torch.dtype = torch.bfloat16, out: torch.T
 def _check_product(a_cols: int, b: FP4Operand, bias, residual, rows: int) -> None:
     if a_cols != b.k:
         raise ValueError(f"the operands contract over {a_cols} and {b.k} values")
-    if bias is not None and tuple(bias.shape) != (b.rows,):
+    if bias is not None and bias.shape != (b.rows,):
         raise ValueError(f"bias must be [{b.rows}]")
-    if residual is not None and tuple(residual.shape) != (rows, b.rows):
+    if residual is not None and residual.shape != (rows, b.rows):
         raise ValueError(f"residual must be [{rows}, {b.rows}]")
 
 
@@ -151,7 +152,7 @@ def gemm(a: FP4Operand, b: FP4Operand, *, bias: torch.Tensor | None = None,
 
 def _linear(x, w: FP4Operand, bias, residual):
     return ext().fp4_linear(x if x.stride(1) == 1 else x.contiguous(), w.data, w.scales, w.row_scale, w.parts,
-                            FORMATS[w.fmt], None if bias is None else compute_view(bias).contiguous(), residual,
+                            FORMATS[w.fmt], None if bias is None else view(bias).contiguous(), residual,
                             status(x.device))
 
 
@@ -192,6 +193,9 @@ def linear_fp4(x: torch.Tensor, weight: FP4Operand, bias: torch.Tensor | None = 
         if residual is not None and residual.dtype != torch.bfloat16:
             raise TypeError("residual must be bfloat16 like x")
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, bias, residual)):
+            if plain(bias) and x.stride(1) == 1 and (bias is None or bias.is_contiguous()):
+                return ext().fp4_linear_apply(x, weight.data, weight.scales, weight.row_scale, weight.parts,
+                                              FORMATS[weight.fmt], bias, residual, status(x.device))
             return LinearFP4Fn.apply(x, weight, bias, residual)
         return _linear(x, weight, bias, residual)
     return linear_fp4_reference(x, weight, bias, residual)
@@ -225,7 +229,7 @@ def gated_feed_forward_fp4(x: torch.Tensor, gate_up: FP4Operand, down: FP4Operan
         return linear_fp4(h, down, down_bias, residual)
     if residual is not None and residual.dtype != torch.bfloat16:
         raise TypeError("residual must be bfloat16 like x")
-    bias = lambda t: None if t is None else compute_view(t).contiguous()  # noqa: E731
+    bias = lambda t: None if t is None else view(t).contiguous()  # noqa: E731
     return ext().fp4_ffn(x if x.stride(1) == 1 else x.contiguous(), gate_up.data, gate_up.scales, gate_up.row_scale,
                          FORMATS[gate_up.fmt], down.data, down.scales, down.row_scale, FORMATS[down.fmt],
                          ACT_CODES[activation], bias(gate_up_bias), bias(down_bias), residual, status(x.device))

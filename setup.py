@@ -24,7 +24,7 @@ SOURCES = [
     "mnr.cu",
     "optim.cu",
     "comm.cu", "pointwise.cu", "gemm_fp8.cu", "int4.cu", "mnr_tc.cu", "mxfp8.cu", "int4_gemm.cu", "attention_bwd_ws.cu", "attention_fwd_ws.cu",
-    "ffn.cpp", "gated.cu", "few_rows.cu", "fp4.cpp", "fp4_quant.cu", "fp4_gemm.cu",
+    "ffn.cpp", "autograd_nodes.cpp", "gated.cu", "few_rows.cu", "fp4.cpp", "fp4_quant.cu", "fp4_gemm.cu",
 ]
 
 NVCC_FLAGS = [
