@@ -44,6 +44,9 @@ setup(
         CUDAExtension(
             name="representax_b200._C",
             sources=[os.path.join(CSRC, s) for s in SOURCES],
+            # The shared C++ runtime that torch uses: a compiler whose own directory lacks it would link a second,
+            # static copy, and an argument check that formats a number would crash in that copy's locale.
+            extra_link_args=["-nostdlib++", "-l:libstdc++.so.6"],
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": NVCC_FLAGS},
         )
     ],
