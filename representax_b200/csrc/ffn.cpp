@@ -246,12 +246,12 @@ std::vector<at::Tensor> gated_ffn_forward(const at::Tensor& x_in, const at::Tens
                                           const OptTensor& gate_up_bias, const OptTensor& down_bias,
                                           const OptTensor& residual_in, int64_t act, bool save, const at::Tensor& status) {
   check_bf16(x_in, "x");
-  check_bf16(gate_up_in, "gate_up");
-  check_bf16(down_in, "down");
-  RX_CHECK(x_in.dim() == 2 && gate_up_in.dim() == 2 && down_in.dim() == 2, "x, gate_up and down must be matrices");
   const int dev = x_in.get_device();
   for (const OptTensor& t : {OptTensor(gate_up_in), OptTensor(down_in), gate_up_bias, down_bias, residual_in})
     RX_CHECK(!t.has_value() || (t->is_cuda() && t->get_device() == dev), "every operand must be on device ", dev, " of x");
+  check_bf16(gate_up_in, "gate_up");
+  check_bf16(down_in, "down");
+  RX_CHECK(x_in.dim() == 2 && gate_up_in.dim() == 2 && down_in.dim() == 2, "x, gate_up and down must be matrices");
   c10::cuda::CUDAGuard guard(dev);
   const at::Tensor x = rows16(x_in), gate_up = rows16(gate_up_in), down = rows16(down_in);
   const OptTensor b1 = vector16(gate_up_bias), b2 = vector16(down_bias);

@@ -57,7 +57,7 @@ def plain(param) -> bool:
 def view(param):
     """The bf16 compute copy of a parameter, or None."""
 
-    return param if plain(param) else computeview(param)
+    return param if plain(param) else compute_view(param)
 
 
 class GatedFeedForwardFn(torch.autograd.Function):
