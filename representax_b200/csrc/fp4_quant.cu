@@ -13,9 +13,10 @@
 //
 // Bound by HBM: x is read once (2 or 4 bytes a value), half a byte a value and
 // the scales are written; the instructions per value are the next limit, so
-//  * a lane takes 8 consecutive values (one or two 16-byte loads, one 4-byte
-//    store) and a warp 256; maxima are taken on the raw 16-bit pairs;
-//  * a warp has kAhead such pieces of its row in flight; NVFP4, whose codes need
+//  * a lane takes 16 consecutive values (32-byte loads, an 8-byte store): an NVFP4
+//    block or half an MXFP4 block, so few lanes work out the same scale; maxima
+//    are taken on the raw 16-bit pairs;
+//  * a warp has kAhead pieces of 512 values in flight; NVFP4, whose codes need
 //    the row's maximum first, reads the row a second time while it is still
 //    in L1 or L2, which beat keeping it in registers (occupancy);
 //  * a quotient by an E4M3 scale is a product with its reciprocal and one
@@ -36,9 +37,17 @@ namespace fp4 {
 
 constexpr int kQuantThreads = 256;
 constexpr int kQuantWarps = kQuantThreads / 32;
-// Pieces of 256 values that a warp has in flight.
+constexpr int kLane = 16, kPiece = 32 * kLane;  // values of a lane and of a warp
+// Pieces that a warp has in flight.
 template <typename T>
-constexpr int kAhead = 8 / sizeof(T);
+constexpr int kAhead = 4 / sizeof(T);
+
+// 32-byte read-only load, issued as written.
+__device__ __forceinline__ void load32(const void* ptr, uint32_t* w) {
+  asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(ptr));
+}
 
 template <typename T>
 __device__ __forceinline__ float to_float(T v) { return static_cast<float>(v); }
@@ -54,30 +63,33 @@ __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bf
 template <>
 __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 
-// Eight consecutive values as loaded: four 32-bit words of 16-bit pairs, or eight fp32 words.
+// A lane's values as loaded: words of 16-bit pairs, or of fp32.
 template <typename T>
 struct Raw {
-  static constexpr int kWords = 2 * sizeof(T);
+  static constexpr int kWords = kLane * sizeof(T) / 4;
   uint32_t w[kWords];
 
-  // Columns c.. of a row: VEC 16-byte loads where all eight exist (always, with FULL), zeros past K.
-  template <bool VEC, bool FULL>
+  // Columns c.. of a row: loads of VEC bytes (0: one by one) where all exist (always, with FULL), zeros past K.
+  template <int VEC, bool FULL>
   __device__ __forceinline__ void load(const T* row, int c, int K) {
-    if (VEC && (FULL || c + 8 <= K)) {
+    if (VEC == 32 && (FULL || c + kLane <= K)) {
 #pragma unroll
-      for (int i = 0; i < kWords / 4; ++i) {
-        const uint4 v = ldg_v4_issue(reinterpret_cast<const uint4*>(row + c) + i);
-        w[4 * i] = v.x;
-        w[4 * i + 1] = v.y;
-        w[4 * i + 2] = v.z;
-        w[4 * i + 3] = v.w;
+      for (int i = 0; i < kWords; i += 8) load32(reinterpret_cast<const uint32_t*>(row + c) + i, w + i);
+    } else if (VEC == 16 && (FULL || c + kLane <= K)) {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 v = ldg_v4_issue(reinterpret_cast<const uint32_t*>(row + c) + i);
+        w[i] = v.x;
+        w[i + 1] = v.y;
+        w[i + 2] = v.z;
+        w[i + 3] = v.w;
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kWords; ++i) w[i] = 0u;
       T* e = reinterpret_cast<T*>(w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < kLane; ++i)
         if (c + i < K) e[i] = row[c + i];
     }
   }
@@ -108,10 +120,10 @@ struct Raw {
       return __float_as_uint(to_float(*reinterpret_cast<const T*>(&h))) & 0x7fffffffu;
     }
   }
-  __device__ __forceinline__ void values(float (&v)[8]) const {
+  __device__ __forceinline__ void values(float (&v)[kLane]) const {
     const T* e = reinterpret_cast<const T*>(w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_float(e[i]);
+    for (int i = 0; i < kLane; ++i) v[i] = to_float(e[i]);
   }
 };
 
@@ -136,7 +148,7 @@ __device__ __forceinline__ float quotient(float a, float s, float inv) {
 // A row belongs to `warps_per_row` warps (1, 2, 4 or 8), which take spans of kAhead pieces in turn; in MXFP4,
 // where spans do not depend on one another, blockIdx.y goes over them instead. All scale bytes of the row
 // tiles are written, those of the padding included.
-template <typename T, int FMT, bool VEC>
+template <typename T, int FMT, int VEC>
 __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantParams p, int warps_per_row) {
   __shared__ uint32_t tops[kQuantWarps];
   grid_launch_dependents();  // a product of these codes may fetch its other operand meanwhile
@@ -151,7 +163,7 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantP
   const int64_t row = part * p.rows + r;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const int extent = static_cast<int>(p.groups) * 4 * block_of(FMT);
-  constexpr int kSpan = kAhead<T> * 256;                               // consecutive columns that a warp takes at a time
+  constexpr int kSpan = kAhead<T> * kPiece;                              // consecutive columns that a warp takes at a time
   const int p0 = (place + blockIdx.y * warps_per_row) * kSpan;        // its first (grid.y is 1 in NVFP4)
   const int stride = warps_per_row * kSpan;
   const int K = live ? p.K : 0;  // rows of the padding hold nothing
@@ -161,12 +173,13 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantP
 #pragma unroll
     for (int i = 0; i < kAhead<T>; ++i) {
       if (full)
-        raw[i].template load<VEC, true>(x, c + lane * 8 + i * 256, K);
+        raw[i].template load<VEC, true>(x, c + lane * kLane + i * kPiece, K);
       else
-        raw[i].template load<VEC, false>(x, c + lane * 8 + i * 256, K);
+        raw[i].template load<VEC, false>(x, c + lane * kLane + i * kPiece, K);
     }
   };
   float factor = 1.f, inv_factor = 1.f;
+  bool fold = true;  // s f and 1 / (s f) are normal numbers for every E4M3 s
   if constexpr (FMT == kNv) {
     uint32_t t = 0;
     for (int c = p0; c < K; c += stride) {
@@ -182,6 +195,7 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantP
     }
     factor = row_factor(top);
     inv_factor = __uint_as_float(0x7f000000u - __float_as_uint(factor));  // 2^-e (any value for a NaN factor)
+    fold = factor >= 0x1p-80f;
     if (live && place == 0 && lane == 0) p.row_scale[row] = factor;
   }
   if (!in_grid) return;
@@ -191,35 +205,43 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantP
   uint8_t* q = p.q + row * p.ldq;
   auto emit = [&](const Raw<T>& in, int c, bool full) {
     uint32_t t = in.top(), byte;
-    float v[8];
+    float v[kLane];
     in.values(v);
-    t = Raw<T>::max_of(t, __shfl_xor_sync(0xffffffffu, t, 1));
     if constexpr (FMT == kMx) {
-      t = Raw<T>::max_of(t, __shfl_xor_sync(0xffffffffu, t, 2));
+      t = Raw<T>::max_of(t, __shfl_xor_sync(0xffffffffu, t, 1));
       byte = mx_scale_byte(Raw<T>::top_bits(t));
       const float inv = mx_inverse(byte);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= inv;
+      for (int i = 0; i < kLane; ++i) v[i] *= inv;
     } else {
       const float want = quotient(__uint_as_float(Raw<T>::top_bits(t)) * inv_factor, 6.f, 1.f / 6.f);
       byte = __nv_cvt_float_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
       // a row with a NaN factor is NaN by that factor whatever its codes; a zero scale has zero codes
-      const float s = e4m3_value(byte), inv = s > 0.f ? __frcp_rn(s) : 0.f;
+      float s = e4m3_value(byte), inv = s > 0.f ? __frcp_rn(s) : 0.f;
+      if (fold) {  // s f and its reciprocal, rounded like that of s: f is a power of two
+        s *= factor;
+        inv *= inv_factor;
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = quotient(v[i] * inv_factor, s, inv);
+        for (int i = 0; i < kLane; ++i) v[i] *= inv_factor;
+      }
+#pragma unroll
+      for (int i = 0; i < kLane; ++i) v[i] = quotient(v[i], s, inv);
     }
-    const uint32_t codes = pack8(v);
+    uint2 codes;
+    codes.x = pack8(reinterpret_cast<const float(&)[8]>(v[0]));
+    codes.y = pack8(reinterpret_cast<const float(&)[8]>(v[8]));
     // four blocks' bytes -> one 4-byte word of the group, written by its first lane
-    constexpr int kLanes = block_of(FMT) / 8;  // lanes of a block
+    constexpr int kLanes = block_of(FMT) / kLane;  // lanes of a block
     uint32_t word = byte << (8 * ((lane / kLanes) & 3));
 #pragma unroll
     for (int o = kLanes; o < 4 * kLanes; o *= 2) word |= __shfl_xor_sync(0xffffffffu, word, o);
     if (full) {
       if (lane % (4 * kLanes) == 0) *reinterpret_cast<uint32_t*>(sf + static_cast<int64_t>(c / (4 * block_of(FMT))) * 512) = word;
-      *reinterpret_cast<uint32_t*>(q + (c >> 1)) = codes;
+      *reinterpret_cast<uint2*>(q + (c >> 1)) = codes;
     } else if (c < extent) {
       if (lane % (4 * kLanes) == 0) *reinterpret_cast<uint32_t*>(sf + static_cast<int64_t>(c / (4 * block_of(FMT))) * 512) = live ? word : 0u;
-      if (live && (c >> 1) < p.ldq) *reinterpret_cast<uint32_t*>(q + (c >> 1)) = codes;
+      if (live && (c >> 1) < p.ldq) *reinterpret_cast<uint2*>(q + (c >> 1)) = codes;
     }
   };
   // (in NVFP4 the row was read just before: its lines are still near)
@@ -228,7 +250,7 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantP
     load_pieces(c, full);
     if (full) {
 #pragma unroll
-      for (int i = 0; i < kAhead<T>; ++i) emit(raw[i], c + i * 256 + lane * 8, true);
+      for (int i = 0; i < kAhead<T>; ++i) emit(raw[i], c + i * kPiece + lane * kLane, true);
     } else {
 #pragma unroll 1
       for (int i = 0; i < kAhead<T>; ++i) {
@@ -236,7 +258,7 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantP
 #pragma unroll
         for (int j = 1; j < kAhead<T>; ++j)
           if (j == i) in = raw[j];
-        if (c + i * 256 < extent) emit(in, c + i * 256 + lane * 8, false);
+        if (c + i * kPiece < extent) emit(in, c + i * kPiece + lane * kLane, false);
       }
     }
     if constexpr (FMT == kMx) break;  // the next columns are another CTA's
@@ -252,16 +274,20 @@ static int row_warps(int64_t rows, int64_t spans) {
 
 template <typename T, int FMT>
 cudaError_t quantize_typed(const QuantParams& p, cudaStream_t stream) {
-  const bool vec = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.ldx % (16 / sizeof(T)) == 0;
+  auto aligned = [&](unsigned bytes) {
+    return reinterpret_cast<uintptr_t>(p.x) % bytes == 0 && p.ldx * static_cast<int64_t>(sizeof(T)) % bytes == 0;
+  };
   const int64_t slots = p.parts * ((p.rows + 127) / 128 * 128);
-  const int64_t extent = p.groups * 4 * block_of(FMT), spans = (extent + kAhead<T> * 256 - 1) / (kAhead<T> * 256);
+  const int64_t extent = p.groups * 4 * block_of(FMT), span = kAhead<T> * kPiece, spans = (extent + span - 1) / span;
   const int wpr = FMT == kMx ? 1 : row_warps(slots, spans);
   const dim3 grid(static_cast<unsigned>((slots * wpr + kQuantWarps - 1) / kQuantWarps),
                   FMT == kMx ? static_cast<unsigned>(spans) : 1u);
-  if (vec)
-    quantize_kernel<T, FMT, true><<<grid, kQuantThreads, 0, stream>>>(p, wpr);
+  if (aligned(32))
+    quantize_kernel<T, FMT, 32><<<grid, kQuantThreads, 0, stream>>>(p, wpr);
+  else if (aligned(16))
+    quantize_kernel<T, FMT, 16><<<grid, kQuantThreads, 0, stream>>>(p, wpr);
   else
-    quantize_kernel<T, FMT, false><<<grid, kQuantThreads, 0, stream>>>(p, wpr);
+    quantize_kernel<T, FMT, 0><<<grid, kQuantThreads, 0, stream>>>(p, wpr);
   return cudaGetLastError();
 }
 
@@ -274,10 +300,21 @@ cudaError_t quantize(const QuantParams& p, int fmt, int type, cudaStream_t strea
   }
 }
 
-// Lane: 16 bytes of output (8 or 4 consecutive values) per piece, so a warp stores 512 contiguous bytes.
+// Eight outputs, as one 16- or 32-byte store.
+template <typename T>
+__device__ __forceinline__ void store8(T* dst, const T (&v)[8]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+  if constexpr (sizeof(T) == 2)
+    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+  else
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
+// A lane decodes eight consecutive values at a time, a warp 256. Rows as in the quantiser.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const DequantParams p, int warps_per_row, bool vec) {
-  constexpr int kVals = 16 / sizeof(T), kPiece = 32 * kVals;
   const int warp = warp_id(), lane = lane_id();
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kQuantWarps / warps_per_row) + warp / warps_per_row;
   if (row >= p.parts * p.rows) return;
@@ -287,9 +324,8 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const Dequant
   const float factor = FMT == kNv ? p.row_scale[row] : 1.f;
   T* out = static_cast<T*>(p.out) + row * p.ldo;
 #pragma unroll 4
-  for (int c = (warp % warps_per_row) * kPiece + lane * kVals; c < p.K; c += warps_per_row * kPiece) {
-    const uint32_t codes = kVals == 8 ? *reinterpret_cast<const uint32_t*>(q + (c >> 1))
-                                      : *reinterpret_cast<const uint16_t*>(q + (c >> 1));
+  for (int c = (warp % warps_per_row) * 256 + lane * 8; c < p.K; c += warps_per_row * 256) {
+    const uint32_t codes = *reinterpret_cast<const uint32_t*>(q + (c >> 1));
     const int block = c / block_of(FMT);
     const uint32_t byte = sf[static_cast<int64_t>(block >> 2) * 512 + (block & 3)];
     float scale;
@@ -299,14 +335,14 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const Dequant
       scale = e4m3_value(byte) * factor;
     float f[8];
     unpack8(codes, f);
-    T v[kVals];
+    T v[8];
 #pragma unroll
-    for (int j = 0; j < kVals; ++j) v[j] = from_float<T>(f[j] * scale);
-    if (vec && c + kVals <= p.K) {
-      *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<const uint4*>(v);
+    for (int j = 0; j < 8; ++j) v[j] = from_float<T>(f[j] * scale);
+    if (vec && c + 8 <= p.K) {
+      store8(out + c, v);
     } else {
 #pragma unroll
-      for (int j = 0; j < kVals; ++j)
+      for (int j = 0; j < 8; ++j)
         if (c + j < p.K) out[c + j] = v[j];
     }
   }
@@ -314,9 +350,10 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const Dequant
 
 template <typename T>
 cudaError_t dequantize_typed(const DequantParams& p, int fmt, cudaStream_t stream) {
-  const bool vec = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo % (16 / sizeof(T)) == 0;
+  constexpr int kAlign = 8 * sizeof(T);
+  const bool vec = reinterpret_cast<uintptr_t>(p.out) % kAlign == 0 && p.ldo % 8 == 0;
   const int64_t rows = p.parts * p.rows;
-  const int wpr = row_warps(rows, p.K / (512 / static_cast<int>(sizeof(T))));
+  const int wpr = row_warps(rows, (p.K + 255) / 256);
   const unsigned grid = static_cast<unsigned>((rows * wpr + kQuantWarps - 1) / kQuantWarps);
   if (fmt == kMx)
     dequantize_kernel<T, kMx><<<grid, kQuantThreads, 0, stream>>>(p, wpr, vec);
