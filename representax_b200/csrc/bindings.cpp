@@ -123,7 +123,7 @@ void gated_forward(const at::Tensor& x, const at::Tensor& gate_up, const c10::op
                    const c10::optional<at::Tensor>& saved, const c10::optional<at::Tensor>& exps, int64_t act,
                    const at::Tensor& status);
 void gated_backward(const at::Tensor& dy, const at::Tensor& down, const at::Tensor& saved, const at::Tensor& exps,
-                    at::Tensor& dz, const at::Tensor& status);
+                    at::Tensor& dz, const c10::optional<at::Tensor>& partial, const at::Tensor& status);
 void few_rows_linear(const at::Tensor& x, const at::Tensor& w, int64_t parts, int64_t act,
                      const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual, at::Tensor& out,
                      bool after_producer, const at::Tensor& status);

@@ -213,8 +213,9 @@ void gated_forward(const at::Tensor& x, const at::Tensor& gate_up, const OptTens
 }
 
 // dz [T, 2 I] = [dh b | dh a] with dh = dy Wd (dy [T, H], down [H, I]) and what gated_forward saved.
+// `partial` (fp32 [ceil(T / 32), 2 I]): also the column sums of dz over each 32 rows.
 void gated_backward(const at::Tensor& dy, const at::Tensor& down, const at::Tensor& saved, const at::Tensor& exps,
-                    at::Tensor& dz, const at::Tensor& status) {
+                    at::Tensor& dz, const OptTensor& partial, const at::Tensor& status) {
   check_bf16(dy, "dy");
   check_bf16(down, "down");
   check_bf16(dz, "dz");
@@ -227,6 +228,12 @@ void gated_backward(const at::Tensor& dy, const at::Tensor& down, const at::Tens
   check_rows(dz, "dz", T, 2 * I, dev);
   check_saved(saved, exps, T, I, dev);
   gated::Params p = make_params(T, I, H, 256, status);
+  if (partial.has_value()) {
+    check_f32(*partial, "partial");
+    RX_CHECK(partial->get_device() == dev && partial->is_contiguous() && partial->numel() == (T + 31) / 32 * 2 * I,
+             "partial must be a contiguous [ceil(T / 32), 2 I]");
+    p.partial = partial->data_ptr<float>();
+  }
   p.saved = reinterpret_cast<uint4*>(saved.data_ptr());
   p.exps = reinterpret_cast<uint16_t*>(exps.data_ptr());
   c10::cuda::CUDAGuard guard(dev);
@@ -298,12 +305,29 @@ std::vector<at::Tensor> gated_ffn_backward(const at::Tensor& dy_in, const OptTen
     RX_CHECK(saved.has_value() && exps.has_value(), "the forward did not save for this gradient");
     const at::Tensor down = rows16(down_in);
     at::Tensor dz = at::empty({dy.size(0), 2 * down.size(1)}, dy.options());
-    gated_backward(dy, down, *saved, *exps, dz, status);
+    at::Tensor partial;
+    if (need[3]) partial = at::empty({(dy.size(0) + 31) / 32, 2 * down.size(1)}, dy.options().dtype(at::kFloat));
+    gated_backward(dy, down, *saved, *exps, dz, need[3] ? OptTensor(partial) : c10::nullopt, status);
     if (need[1]) {
       RX_CHECK(x.has_value(), "the gradient of gate_up needs x");
       out[1] = weight_gradient(dz, rows16(*x), acc[1], like[1], status);
     }
-    if (need[3]) out[3] = bias_gradient(dz, acc[3], like[3]);
+    if (need[3]) {
+      const int64_t cols = partial.size(1);
+      const bool direct = !acc[3].has_value() && like[3] == at::kBFloat16;
+      if (acc[3].has_value()) {
+        check_f32(*acc[3], "accumulator");
+        RX_CHECK(acc[3]->is_contiguous() && acc[3]->numel() == cols, "accumulator must be a contiguous vector of ", cols);
+      }
+      at::Tensor db = direct ? at::empty({cols}, dy.options())
+                             : (acc[3].has_value() ? *acc[3] : at::zeros({cols}, dy.options().dtype(at::kFloat)));
+      const cudaError_t e = gated::sum_partials(
+          partial.data_ptr<float>(), partial.size(0), cols, direct ? nullptr : db.data_ptr<float>(),
+          direct ? reinterpret_cast<__nv_bfloat16*>(db.data_ptr()) : nullptr,
+          at::cuda::getCurrentCUDAStream(dy.get_device()).stream());
+      RX_CHECK(e == cudaSuccess, "gated feed-forward: ", cudaGetErrorString(e));
+      if (!acc[3].has_value()) out[3] = direct || like[3] == at::kFloat ? db : db.to(like[3]);
+    }
     if (need[0]) {
       const at::Tensor gate_up = rows16(gate_up_in);
       out[0] = at::empty({dy.size(0), gate_up.size(1)}, dy.options());

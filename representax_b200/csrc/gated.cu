@@ -26,7 +26,9 @@
 //
 // Backward: the input-gradient GEMM dy Wd with 256 x 256 pair tiles whose
 // epilogue reads the saved tiles (prefetched one 32-column chunk ahead) and
-// stores the two halves of dz; dh is never written.
+// stores the two halves of dz; dh is never written. With biases it also leaves
+// the column sums of each 32 rows, which a second launch adds up in a fixed
+// order (the sums of a separate pass over dz took longer than dz itself).
 //
 // Both are bound by the tensor pipe at training sizes (see the figures at the
 // host entries). The main loops follow the pair kernel of gemm_kernel.cuh: five
@@ -119,6 +121,20 @@ __device__ __forceinline__ void add_bias32(const __nv_bfloat16* bias, int n_base
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] += n_base + i < n ? __bfloat162float(bias[n_base + i]) : 0.f;
   }
+}
+
+// Sum over the warp's lanes (rows) of each of 32 columns; lane c returns column c's.
+__device__ __forceinline__ float column_sum32(float (&v)[32], int lane) {
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) {
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const bool high = (lane & o) != 0;
+      const float send = high ? v[i] : v[i + o], keep = high ? v[i + o] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+  return v[0];
 }
 
 // Index of the saved tile that holds rows row0.. (of 32) and columns n.. (of 32).
@@ -335,6 +351,15 @@ __global__ void __launch_bounds__(kThreads, 1)
               times_row32(cur_a, load_factor(e >> 8), r, v);
             gemm::stage_row32_sw64(buf, lane, v);
             store_tile32(buf, p.out[half], p.ld_out, row0, n, p.M, p.N, lane);
+            if (p.partial != nullptr) {  // the bias gradient, from the values before their rounding
+              if (row0 + lane >= p.M) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = 0.f;
+              }
+              const float sum = column_sum32(v, lane);
+              if (n + lane < p.N)
+                p.partial[(static_cast<int64_t>(row0 >> 5) * 2 + half) * p.N + n + lane] = sum;
+            }
           }
         } else {
           uint32_t rg[32], ru[32];
@@ -391,6 +416,33 @@ gate_and_keep(p.act, g, v, b);
   cluster_sync_all();  // no CTA leaves while its peer may still signal it
   tc_fence_after();
   if (warp == 1) tmem_dealloc_pair(tmem_base, kTmemCols);
+}
+
+// 32 columns x 8 row lanes; a column's rows are added in the same order every time.
+__global__ void __launch_bounds__(256) sum_partials_kernel(const float* partial, int rows, int64_t cols, float* acc,
+                                                           __nv_bfloat16* out) {
+  __shared__ float part[8][32];
+  const int lane = lane_id(), w = warp_id();
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  float sum = 0.f;
+  if (c < cols)
+    for (int r = w; r < rows; r += 8) sum += partial[r * cols + c];
+  part[w][lane] = sum;
+  __syncthreads();
+  if (w != 0 || c >= cols) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) sum += part[i][lane];
+  if (acc != nullptr)
+    acc[c] += sum;
+  else
+    out[c] = __float2bfloat16_rn(sum);
+}
+
+cudaError_t sum_partials(const float* partial, int64_t rows, int64_t cols, float* acc, __nv_bfloat16* out,
+                         cudaStream_t stream) {
+  sum_partials_kernel<<<static_cast<unsigned>((cols + 31) / 32), 256, 0, stream>>>(partial, static_cast<int>(rows), cols, acc,
+                                                                                   out);
+  return cudaGetLastError();
 }
 
 template <int MODE>

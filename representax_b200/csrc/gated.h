@@ -20,6 +20,7 @@ struct Params {
   int64_t ld_out;
   uint4* saved;               // [ceil(M / 32)][ceil(N / 32)] tiles of 32 x 32 fp16: b, then a (4 KB)
   uint16_t* exps;             // [the same tiles][32]: low byte the block exponent of b, high byte that of a
+  float* partial;             // backward: [ceil(M / 32)][2 N] column sums of 32 rows of dz, or null
   int* status;
   uint64_t timeout_ns;
 };
@@ -28,6 +29,11 @@ struct Params {
 struct Maps {
   CUtensorMap a, b;
 };
+
+// Column sums of `rows` rows of partial sums [rows][cols], in a fixed order: added to acc (fp32), or written
+// to out (bf16).
+cudaError_t sum_partials(const float* partial, int64_t rows, int64_t cols, float* acc, __nv_bfloat16* out,
+                         cudaStream_t stream);
 
 cudaError_t launch(int mode, const Maps& maps, const Params& p, int sms, int device, cudaStream_t stream);
 
