@@ -21,6 +21,15 @@
 // accumulator, an epilogue thread takes its 128 values into registers and
 // frees the accumulator before it computes or stores, so the tensor core waits
 // for a TMEM read only. bf16 results leave through shared memory and TMA tile stores.
+//
+// What measuring led here (12288 x 8192 outputs, K 2048): with `lane == 0` around the issuing
+// loop every operand of an instruction was moved to uniform registers again, 60 to
+// 90 cycles an instruction, 16 of them a stage: 128 us MXFP4 and 179 us NVFP4
+// against 110 and 121 us with the warp-uniform loop. What bounds it now is the
+// L2: without an epilogue the loads run at 12 TB/s over all SMs, 5.4 PFLOP/s;
+// the epilogue's stores come on top. K 6144, 8192 x 2048 outputs + residual:
+// 53 us MXFP4 (3.9 PFLOP/s), 59 us NVFP4; gated, K 2048, 8192 x 6144 outputs as
+// MXFP4 codes: 97 us (4.3 PFLOP/s).
 #include "fp4.h"
 
 #include <algorithm>
@@ -164,8 +173,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const int num_units = p.m_tiles * p.n_tiles;
 
   if (warp >= kFirstEpi) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
     // ------------------------------------------------------------ epilogue (both CTAs)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
     const int quad = warp & 3, half = (warp - kFirstEpi) >> 2;
     const uint32_t tempty_leader = mapa_shared(smem_u32(tempty), 0);
     uint8_t* const staging = sC + (warp - kFirstEpi) * 4096;
@@ -288,137 +297,137 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     __syncwarp();
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      tma_prefetch_map(&tmA);
-      tma_prefetch_map(&tmB);
-      tma_prefetch_map(&tmSfA);
-      tma_prefetch_map(&tmSfB);
-      const uint32_t full_leader0 = mapa_shared(smem_u32(&full[0]), 0);
-      const int groups = static_cast<int>(p.groups);
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int u = cluster; ok && u < num_units; u += clusters) {
-        const int mt = u % p.m_tiles, nt = u / p.m_tiles;
-        const int m_row = mt * 256 + rank * 128;
-        const int b_row = GATED ? nt * 128 + rank * p.N : nt * 256 + rank * 128;
-        // scale row tiles (a tile past the end reads the last one's: its products are dropped)
-        const int ta = min(2 * mt + rank, p.a_tiles - 1);
-        const int tb0 = GATED ? nt : 2 * nt, tb1 = GATED ? nt + p.b_tiles : min(2 * nt + 1, p.b_tiles - 1);
-        for (int ks = 0; ks < p.k_stages; ++ks) {
-          if (*abort_flag || !mbar_wait(&empty[stage], phase ^ 1, p.timeout_ns)) {
-            report_status(p.status, kStatusTimeoutProducer);
-            *abort_flag = 1;
-            ok = false;
+    if (warp == 0) {
+      // ------------------------------------------------------------ producer
+      if (lane == 0) {
+        tma_prefetch_map(&tmA);
+        tma_prefetch_map(&tmB);
+        tma_prefetch_map(&tmSfA);
+        tma_prefetch_map(&tmSfB);
+        const uint32_t full_leader0 = mapa_shared(smem_u32(&full[0]), 0);
+        const int groups = static_cast<int>(p.groups);
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int u = cluster; ok && u < num_units; u += clusters) {
+          const int mt = u % p.m_tiles, nt = u / p.m_tiles;
+          const int m_row = mt * 256 + rank * 128;
+          const int b_row = GATED ? nt * 128 + rank * p.N : nt * 256 + rank * 128;
+          // scale row tiles (a tile past the end reads the last one's: its products are dropped)
+          const int ta = min(2 * mt + rank, p.a_tiles - 1);
+          const int tb0 = GATED ? nt : 2 * nt, tb1 = GATED ? nt + p.b_tiles : min(2 * nt + 1, p.b_tiles - 1);
+          for (int ks = 0; ks < p.k_stages; ++ks) {
+            if (*abort_flag || !mbar_wait(&empty[stage], phase ^ 1, p.timeout_ns)) {
+              report_status(p.status, kStatusTimeoutProducer);
+              *abort_flag = 1;
+              ok = false;
+              break;
+            }
+            if (leader) mbar_arrive_expect_tx(&full[stage], 2 * S::kStage);  // both CTAs' loads
+            const uint32_t bar = full_leader0 + stage * 8;
+            uint8_t* tiles = base + stage * 2 * kTile;
+            uint8_t* sf = sf_base + stage * S::kSf;
+            constexpr int kBytes = S::kGroups * 512;
+            const int g = ks * S::kGroups;
+            tma_load_2d_pair(tiles, &tmA, bar, ks * 128, m_row);
+            tma_load_2d_pair(tiles + kTile, &tmB, bar, ks * 128, b_row);
+            tma_load_2d_pair(sf, &tmSfA, bar, 0, ta * groups + g);
+            tma_load_2d_pair(sf + kBytes, &tmSfB, bar, 0, tb0 * groups + g);
+            tma_load_2d_pair(sf + 2 * kBytes, &tmSfB, bar, 0, tb1 * groups + g);
+            if (++stage == kGemmStages) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+        }
+        // every load was consumed once the MMAs of its stage have committed
+        for (int s = 0; s < kGemmStages; ++s) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, p.timeout_ns)) {
+            report_status(p.status, kStatusTimeoutDrain);
             break;
           }
-          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * S::kStage);  // both CTAs' loads
-          const uint32_t bar = full_leader0 + stage * 8;
-          uint8_t* tiles = base + stage * 2 * kTile;
-          uint8_t* sf = sf_base + stage * S::kSf;
-          constexpr int kBytes = S::kGroups * 512;
-          const int g = ks * S::kGroups;
-          tma_load_2d_pair(tiles, &tmA, bar, ks * 128, m_row);
-          tma_load_2d_pair(tiles + kTile, &tmB, bar, ks * 128, b_row);
-          tma_load_2d_pair(sf, &tmSfA, bar, 0, ta * groups + g);
-          tma_load_2d_pair(sf + kBytes, &tmSfB, bar, 0, tb0 * groups + g);
-          tma_load_2d_pair(sf + 2 * kBytes, &tmSfB, bar, 0, tb1 * groups + g);
           if (++stage == kGemmStages) {
             stage = 0;
             phase ^= 1;
           }
         }
       }
-      // every load was consumed once the MMAs of its stage have committed
-      for (int s = 0; s < kGemmStages; ++s) {
-        if (!mbar_wait(&empty[stage], phase ^ 1, p.timeout_ns)) {
-          report_status(p.status, kStatusTimeoutDrain);
-          break;
-        }
-        if (++stage == kGemmStages) {
-          stage = 0;
-          phase ^= 1;
-        }
-      }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer (even CTA)
-    if (leader) {
-      // The whole warp runs this loop and one lane issues. What the issuing costs bounds the stage, so its
-      // instructions are kept few: descriptors are a base plus an offset in their address field, and the abort
-      // flag is read only where a wait is not over at once.
-      const uint64_t a0 = smem_desc_sw128(smem_u32(base), 16, 1024);
-      const uint64_t f0 = smem_desc_plain(smem_u32(sf_base), 512, 128);
-      const uint32_t tmem_sf = tmem_base + 256;
-      auto ready = [&](uint64_t* bar, uint32_t parity) -> bool {
-        const bool now = mbar_try_wait(bar, parity) || (*abort_flag == 0 && mbar_wait(bar, parity, p.timeout_ns));
-        return __all_sync(0xffffffffu, now);
-      };
-      // Wait for a stage's data and copy its scales into the stage's TMEM columns.
-      auto fetch = [&](int s, uint32_t phase) -> bool {
-        if (!ready(&full[s], phase)) return false;
-        tc_fence_after();
-        const uint64_t f = f0 + static_cast<uint32_t>(s * (S::kSf >> 4));
-        const uint32_t sfa = tmem_sf + s * S::kSfCols, sfb = sfa + 4 * S::kGroups;
-        if (elect_one()) {
-#pragma unroll
-          for (int j = 0; j < S::kGroups; ++j) {
-            tmem_cp_scales_pair(sfa + 4 * j, f + 32 * j);
-            tmem_cp_scales_pair(sfb + 8 * j, f + 32 * (S::kGroups + j));
-            tmem_cp_scales_pair(sfb + 8 * j + 4, f + 32 * (2 * S::kGroups + j));
-          }
-        }
-        return true;
-      };
-      auto products = [&](int s, int kk, uint32_t accumulate) {
-        const uint64_t a = a0 + static_cast<uint32_t>(s * (2 * kTile >> 4) + kk * 2);
-        const uint32_t sfa = tmem_sf + s * S::kSfCols, sfb = sfa + 4 * S::kGroups;
-        const int atom = FMT == kMx ? kk >> 1 : kk;
-        const uint32_t id = FMT == kMx ? 2u * (kk & 1) : 0u;
-        umma_pair<FMT>(tmem_base, a, a + (kTile >> 4), idesc(256, 256, FMT, id), (sfa + 4 * atom) | (id << 30),
-                       (sfb + 8 * atom) | (id << 30), accumulate);
-      };
-      const int tail = (p.K - (p.k_stages - 1) * kStageK + 63) / 64;  // 64-value steps of the last stage
-      int s = 0, local = 0;
-      uint32_t phase = 0;
-      bool ok = cluster >= num_units || fetch(0, 0);
-      for (int u = cluster; ok && u < num_units; u += clusters, ++local) {
-        ok = ready(tempty, static_cast<uint32_t>(local & 1) ^ 1u);
-        tc_fence_after();
-        for (int ks = 0; ok && ks < p.k_stages; ++ks) {
-          int s1 = s + 1;
-          if (s1 == kGemmStages) {
-            s1 = 0;
-            phase ^= 1;
-          }
-          const bool last = ks + 1 == p.k_stages;
-          if (!last || u + clusters < num_units) ok = fetch(s1, phase);  // one stage ahead
-          if (!ok) break;
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer (even CTA)
+      if (leader) {
+        // The whole warp runs this loop and one lane issues. What the issuing costs bounds the stage, so its
+        // instructions are kept few: descriptors are a base plus an offset in their address field, and the abort
+        // flag is read only where a wait is not over at once.
+        const uint64_t a0 = smem_desc_sw128(smem_u32(base), 16, 1024);
+        const uint64_t f0 = smem_desc_plain(smem_u32(sf_base), 512, 128);
+        const uint32_t tmem_sf = tmem_base + 256;
+        auto ready = [&](uint64_t* bar, uint32_t parity) -> bool {
+          const bool now = mbar_try_wait(bar, parity) || (*abort_flag == 0 && mbar_wait(bar, parity, p.timeout_ns));
+          return __all_sync(0xffffffffu, now);
+        };
+        // Wait for a stage's data and copy its scales into the stage's TMEM columns.
+        auto fetch = [&](int s, uint32_t phase) -> bool {
+          if (!ready(&full[s], phase)) return false;
+          tc_fence_after();
+          const uint64_t f = f0 + static_cast<uint32_t>(s * (S::kSf >> 4));
+          const uint32_t sfa = tmem_sf + s * S::kSfCols, sfb = sfa + 4 * S::kGroups;
           if (elect_one()) {
-            if (!last || tail == 4) {
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk) products(s, kk, (ks > 0 || kk > 0) ? 1u : 0u);
-            } else {  // steps past K would multiply zeros by scales that nothing defines
-              for (int kk = 0; kk < tail; ++kk) products(s, kk, (ks > 0 || kk > 0) ? 1u : 0u);
+            for (int j = 0; j < S::kGroups; ++j) {
+              tmem_cp_scales_pair(sfa + 4 * j, f + 32 * j);
+              tmem_cp_scales_pair(sfb + 8 * j, f + 32 * (S::kGroups + j));
+              tmem_cp_scales_pair(sfb + 8 * j + 4, f + 32 * (2 * S::kGroups + j));
             }
-            umma_commit_pair(&empty[s], 0x3);
-            if (last) umma_commit_pair(tfull, 0x3);
           }
-          __syncwarp();
-          s = s1;
+          return true;
+        };
+        auto products = [&](int s, int kk, uint32_t accumulate) {
+          const uint64_t a = a0 + static_cast<uint32_t>(s * (2 * kTile >> 4) + kk * 2);
+          const uint32_t sfa = tmem_sf + s * S::kSfCols, sfb = sfa + 4 * S::kGroups;
+          const int atom = FMT == kMx ? kk >> 1 : kk;
+          const uint32_t id = FMT == kMx ? 2u * (kk & 1) : 0u;
+          umma_pair<FMT>(tmem_base, a, a + (kTile >> 4), idesc(256, 256, FMT, id), (sfa + 4 * atom) | (id << 30),
+                         (sfb + 8 * atom) | (id << 30), accumulate);
+        };
+        const int tail = (p.K - (p.k_stages - 1) * kStageK + 63) / 64;  // 64-value steps of the last stage
+        int s = 0, local = 0;
+        uint32_t phase = 0;
+        bool ok = cluster >= num_units || fetch(0, 0);
+        for (int u = cluster; ok && u < num_units; u += clusters, ++local) {
+          ok = ready(tempty, static_cast<uint32_t>(local & 1) ^ 1u);
+          tc_fence_after();
+          for (int ks = 0; ok && ks < p.k_stages; ++ks) {
+            int s1 = s + 1;
+            if (s1 == kGemmStages) {
+              s1 = 0;
+              phase ^= 1;
+            }
+            const bool last = ks + 1 == p.k_stages;
+            if (!last || u + clusters < num_units) ok = fetch(s1, phase);  // one stage ahead
+            if (!ok) break;
+            if (elect_one()) {
+              if (!last || tail == 4) {
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) products(s, kk, (ks > 0 || kk > 0) ? 1u : 0u);
+              } else {  // steps past K would multiply zeros by scales that nothing defines
+                for (int kk = 0; kk < tail; ++kk) products(s, kk, (ks > 0 || kk > 0) ? 1u : 0u);
+              }
+              umma_commit_pair(&empty[s], 0x3);
+              if (last) umma_commit_pair(tfull, 0x3);
+            }
+            __syncwarp();
+            s = s1;
+          }
         }
+        if (!ok) {
+          if (lane == 0) report_status(p.status, kStatusTimeoutMma);
+          *abort_flag = 1;
+        }
+        if (elect_one()) umma_commit_pair(drain, 0x3);
       }
-      if (!ok) {
-        if (lane == 0) report_status(p.status, kStatusTimeoutMma);
-        *abort_flag = 1;
-      }
-      if (elect_one()) umma_commit_pair(drain, 0x3);
+      if (lane == 0 && !mbar_wait(drain, 0, p.timeout_ns)) report_status(p.status, kStatusTimeoutDrain);
+      __syncwarp();
     }
-    if (lane == 0 && !mbar_wait(drain, 0, p.timeout_ns)) report_status(p.status, kStatusTimeoutDrain);
-    __syncwarp();
-  }
   }
 
   tc_fence_before();

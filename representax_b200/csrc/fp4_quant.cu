@@ -23,6 +23,9 @@
 //    correction step (Markstein, "Computation of elementary functions on the
 //    IBM RISC System/6000 processor", 1990): the correctly rounded quotient
 //    in three operations, so ties fall as the definition says.
+// [8192, 6144] bf16: MXFP4 25 us (127 MB, 5.0 TB/s), NVFP4 36 us (3.6 TB/s: twice the
+// instructions a value); [12283, 2048] fp32: 19 us (6.1 TB/s) and 27 us; decoding
+// that to fp32 24 us (114 MB, 4.7 TB/s).
 #include "fp4.h"
 
 #include <cuda_fp16.h>
