@@ -2,6 +2,8 @@
 // and the block's forward and backward as one call each (its launches in a row,
 // intermediates from the caching allocator on the current stream), so that a
 // small call is not bound by the host.
+#include <ATen/cuda/EmptyTensor.h>
+
 #include "common.h"
 #include "few_rows.h"
 #include "gated.h"
@@ -18,6 +20,12 @@ void colsum_accumulate(const at::Tensor& x, at::Tensor& out);
 namespace {
 
 using OptTensor = c10::optional<at::Tensor>;
+
+// Uninitialised device memory straight from the CUDA allocator (at::empty without the dispatcher's share of the
+// host time).
+at::Tensor device_empty(at::IntArrayRef sizes, at::ScalarType dtype, int device) {
+  return at::detail::empty_cuda(sizes, dtype, at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device)), c10::nullopt);
+}
 
 // The epilogue and output codes of gemm_kernel.cuh.
 constexpr int64_t kBias = 1, kResidual = 8;
@@ -106,7 +114,7 @@ at::Tensor weight_gradient(const at::Tensor& dy, const at::Tensor& x, const OptT
   // Rounded once in the product's epilogue when its tiles (or a short contraction) leave nothing
   // for a split of K to gain over clearing, adding into and casting an fp32 buffer.
   if (dtype == at::kBFloat16 && (2 * tiles >= num_sms(dy.get_device()) / 2 || k_blocks <= 32)) {
-    at::Tensor out = at::empty({m, n}, dy.options());
+    at::Tensor out = device_empty({m, n}, at::kBFloat16, dy.get_device());
     product(out, kOutBf16);
     return out;
   }
@@ -264,11 +272,11 @@ std::vector<at::Tensor> gated_ffn_forward(const at::Tensor& x_in, const at::Tens
   const OptTensor b1 = vector16(gate_up_bias), b2 = vector16(down_bias);
   const OptTensor residual = residual_in.has_value() ? OptTensor(rows16(*residual_in)) : residual_in;
   const int64_t T = x.size(0), I = down.size(1), H = down.size(0);
-  at::Tensor h = at::empty({T, I}, x.options()), y = at::empty({T, H}, x.options()), saved, exps;
+  at::Tensor h = device_empty({T, I}, at::kBFloat16, dev), y = device_empty({T, H}, at::kBFloat16, dev), saved, exps;
   const bool few_gated = !save && few::takes(T, I, true), few_down = few::takes(T, H, false);
   if (save) {
-    saved = at::empty({saved_tiles(T, I), 2, 32, 32}, x.options().dtype(at::kHalf));
-    exps = at::empty({saved_tiles(T, I), 32}, x.options().dtype(at::kShort));
+    saved = device_empty({saved_tiles(T, I), 2, 32, 32}, at::kHalf, dev);
+    exps = device_empty({saved_tiles(T, I), 32}, at::kShort, dev);
     gated_forward(x, gate_up, b1, h, saved, exps, act, status);
   } else if (few_gated) {
     few_rows_linear(x, gate_up, 2, act, b1, c10::nullopt, h, false, status);
@@ -304,9 +312,9 @@ std::vector<at::Tensor> gated_ffn_backward(const at::Tensor& dy_in, const OptTen
   if (need[0] || need[1] || need[3]) {
     RX_CHECK(saved.has_value() && exps.has_value(), "the forward did not save for this gradient");
     const at::Tensor down = rows16(down_in);
-    at::Tensor dz = at::empty({dy.size(0), 2 * down.size(1)}, dy.options());
+    at::Tensor dz = device_empty({dy.size(0), 2 * down.size(1)}, at::kBFloat16, dy.get_device());
     at::Tensor partial;
-    if (need[3]) partial = at::empty({(dy.size(0) + 31) / 32, 2 * down.size(1)}, dy.options().dtype(at::kFloat));
+    if (need[3]) partial = device_empty({(dy.size(0) + 31) / 32, 2 * down.size(1)}, at::kFloat, dy.get_device());
     gated_backward(dy, down, *saved, *exps, dz, need[3] ? OptTensor(partial) : c10::nullopt, status);
     if (need[1]) {
       RX_CHECK(x.has_value(), "the gradient of gate_up needs x");
@@ -319,7 +327,7 @@ std::vector<at::Tensor> gated_ffn_backward(const at::Tensor& dy_in, const OptTen
         check_f32(*acc[3], "accumulator");
         RX_CHECK(acc[3]->is_contiguous() && acc[3]->numel() == cols, "accumulator must be a contiguous vector of ", cols);
       }
-      at::Tensor db = direct ? at::empty({cols}, dy.options())
+      at::Tensor db = direct ? device_empty({cols}, at::kBFloat16, dy.get_device())
                              : (acc[3].has_value() ? *acc[3] : at::zeros({cols}, dy.options().dtype(at::kFloat)));
       const cudaError_t e = gated::sum_partials(
           partial.data_ptr<float>(), partial.size(0), cols, direct ? nullptr : db.data_ptr<float>(),
@@ -330,7 +338,7 @@ std::vector<at::Tensor> gated_ffn_backward(const at::Tensor& dy_in, const OptTen
     }
     if (need[0]) {
       const at::Tensor gate_up = rows16(gate_up_in);
-      out[0] = at::empty({dy.size(0), gate_up.size(1)}, dy.options());
+      out[0] = device_empty({dy.size(0), gate_up.size(1)}, at::kBFloat16, dy.get_device());
       gemm_tcgen05(dz, gate_up, out[0], false, true, 0, kOutBf16, 1.0, c10::nullopt, c10::nullopt, c10::nullopt,
                    c10::nullopt, status, 0, 0, 0, 0, 0.0, c10::nullopt);
     }

@@ -2,6 +2,8 @@
 // token rows: argument checks, tensor maps, dispatch.
 #include "fp4.h"
 
+#include <ATen/cuda/EmptyTensor.h>
+
 #include "common.h"
 #include "few_rows.h"
 
@@ -16,6 +18,12 @@ void gemm_tcgen05(const at::Tensor& A, const at::Tensor& B, at::Tensor& C, bool 
 namespace {
 
 using OptTensor = c10::optional<at::Tensor>;
+
+// Uninitialised device memory straight from the CUDA allocator (at::empty without the dispatcher's share of the
+// host time).
+at::Tensor device_empty(at::IntArrayRef sizes, at::ScalarType dtype, int device) {
+  return at::detail::empty_cuda(sizes, dtype, at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device)), c10::nullopt);
+}
 
 constexpr int kMx = 1, kNv = 2;
 
@@ -92,10 +100,10 @@ Operand operand(const at::Tensor& q, const at::Tensor& sf, const OptTensor& row_
 struct Workspace {
   at::Tensor memory;
   Operand op;
-  Workspace(int64_t rows, int64_t K, int fmt, const at::TensorOptions& device) {
+  Workspace(int64_t rows, int64_t K, int fmt, int device) {
     op = Operand{nullptr, (K + 31) / 32 * 16, nullptr, nullptr, rows, 1, K, fmt};
     const int64_t codes = rows * op.ldq, scales = op.scale_bytes();
-    memory = at::empty({codes + scales + (fmt == kNv ? 4 * rows : 0)}, device.dtype(at::kByte));
+    memory = device_empty({codes + scales + (fmt == kNv ? 4 * rows : 0)}, at::kByte, device);
     op.q = memory.data_ptr<uint8_t>();
     op.sf = op.q + codes;
     if (fmt == kNv) op.row = reinterpret_cast<float*>(op.sf + scales);
@@ -298,11 +306,10 @@ std::vector<at::Tensor> fp4_quantize(const at::Tensor& x, int64_t parts, int64_t
   const int64_t rows = x.size(0) / parts, K = x.size(1);
   const int dev = x.get_device();
   c10::cuda::CUDAGuard guard(dev);
-  const auto bytes = x.options().dtype(at::kByte);
-  at::Tensor q = at::empty({x.size(0), (K + 31) / 32 * 16}, bytes);
-  at::Tensor sf = at::empty({parts * row_tiles(rows), scale_groups(K, fmt), 512}, bytes);
+  at::Tensor q = device_empty({x.size(0), (K + 31) / 32 * 16}, at::kByte, dev);
+  at::Tensor sf = device_empty({parts * row_tiles(rows), scale_groups(K, fmt), 512}, at::kByte, dev);
   at::Tensor row;
-  if (fmt == kNv) row = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+  if (fmt == kNv) row = device_empty({x.size(0)}, at::kFloat, dev);
   const Operand o = operand(q, sf, fmt == kNv ? OptTensor(row) : c10::nullopt, parts, K, fmt, dev, "quantize");
   run_quantize(x, o, at::cuda::getCurrentCUDAStream(dev).stream());
   return {q, sf, row};
@@ -327,7 +334,7 @@ at::Tensor fp4_gemm(const at::Tensor& a, const at::Tensor& a_sf, const OptTensor
   const int dev = a.get_device();
   const Operand oa = operand(a, a_sf, a_row, 1, K, fmt, dev, "a"), ob = operand(b, b_sf, b_row, parts, K, fmt, dev, "b");
   c10::cuda::CUDAGuard guard(dev);
-  at::Tensor out = at::empty({oa.rows, ob.all_rows()}, a.options().dtype(at::kBFloat16));
+  at::Tensor out = device_empty({oa.rows, ob.all_rows()}, at::kBFloat16, dev);
   run_linear(oa, ob, bias, unit_rows(residual), out, false, status, dev, at::cuda::getCurrentCUDAStream(dev).stream());
   return out;
 }
@@ -341,8 +348,8 @@ at::Tensor fp4_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor
   const Operand ow = operand(w, w_sf, w_row, parts, x.size(1), fmt, dev, "weight");
   c10::cuda::CUDAGuard guard(dev);
   auto stream = at::cuda::getCurrentCUDAStream(dev).stream();
-  at::Tensor out = at::empty({x.size(0), ow.all_rows()}, x.options());
-  const Workspace xq(x.size(0), x.size(1), ow.fmt, x.options());
+  at::Tensor out = device_empty({x.size(0), ow.all_rows()}, at::kBFloat16, dev);
+  const Workspace xq(x.size(0), x.size(1), ow.fmt, dev);
   run_quantize(x, xq.op, stream);
   run_linear(xq.op, ow, bias, unit_rows(residual), out, true, status, dev, stream);
   return out;
@@ -360,13 +367,13 @@ at::Tensor fp4_linear_dgrad(const at::Tensor& dy_in, const at::Tensor& w, const 
   if (M == 0 || N == 0) return at::zeros({M, K}, dy_in.options());
   at::Tensor dy = dy_in;
   if (!(dy.stride(1) == 1 && dy.stride(0) >= N && aligned_rows(dy))) {  // rows that the tensor map can read
-    dy = at::empty({M, (N + 7) / 8 * 8}, dy_in.options()).narrow(1, 0, N);
+    dy = device_empty({M, (N + 7) / 8 * 8}, at::kBFloat16, dev).narrow(1, 0, N);
     dy.copy_(dy_in);
   }
   const int64_t ld = (K + 7) / 8 * 8;
-  at::Tensor wide = at::empty({N, ld}, dy.options()).narrow(1, 0, K);
+  at::Tensor wide = device_empty({N, ld}, at::kBFloat16, dev).narrow(1, 0, K);
   run_dequantize(ow, wide, at::cuda::getCurrentCUDAStream(dev).stream());
-  at::Tensor dx = at::empty({M, ld}, dy.options()).narrow(1, 0, K);
+  at::Tensor dx = device_empty({M, ld}, at::kBFloat16, dev).narrow(1, 0, K);
   gemm_tcgen05(dy, wide, dx, false, true, 0, 0, 1.0, c10::nullopt, c10::nullopt, c10::nullopt, c10::nullopt, status, 0, 0, 0,
                0, 0.0, c10::nullopt);
   return dx;
@@ -387,13 +394,13 @@ at::Tensor fp4_ffn(const at::Tensor& x, const at::Tensor& gu, const at::Tensor& 
   c10::cuda::CUDAGuard guard(dev);
   auto stream = at::cuda::getCurrentCUDAStream(dev).stream();
   const int64_t M = x.size(0);
-  at::Tensor y = at::empty({M, od.rows}, x.options());
-  const Workspace xq(M, x.size(1), og.fmt, x.options()), hq(M, og.rows, od.fmt, x.options());
+  at::Tensor y = device_empty({M, od.rows}, at::kBFloat16, dev);
+  const Workspace xq(M, x.size(1), og.fmt, dev), hq(M, og.rows, od.fmt, dev);
   run_quantize(x, xq.op, stream);
   if (og.fmt == kMx && od.fmt == kMx) {
     run_product(xq.op, og, act, gu_bias, c10::nullopt, nullptr, &hq.op, true, status, dev, stream);
   } else {
-    const at::Tensor h = at::empty({M, og.rows}, x.options());
+    const at::Tensor h = device_empty({M, og.rows}, at::kBFloat16, dev);
     run_product(xq.op, og, act, gu_bias, c10::nullopt, &h, nullptr, true, status, dev, stream);
     run_quantize(h, hq.op, stream);
   }

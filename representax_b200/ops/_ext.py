@@ -52,6 +52,7 @@ class _CountingModule:
                 self.launches += weight
             return fn(*args, **kwargs)
 
+        self.__dict__[name] = wrapped  # found without __getattr__ from now on
         return wrapped
 
 

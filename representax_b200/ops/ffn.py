@@ -23,16 +23,12 @@ import torch
 
 from ._ext import ext, status
 from .functional import compute_view
-
-
-def _codes() -> dict[str, int]:
-    from .nn import ACT_CODES
-
-    return ACT_CODES
+from .nn import ACT_CODES as _CODES
+from .nn import _act_reference
 
 
 def _check(x, gate_up, down, activation, gate_up_bias, down_bias, residual) -> None:
-    if activation not in _codes():
+    if activation not in _CODES:
         raise ValueError(f"unsupported activation {activation!r}")
     if x.dim() != 2 or gate_up.dim() != 2 or down.dim() != 2:
         raise ValueError("x, gate_up and down must be matrices")
@@ -46,6 +42,13 @@ def _check(x, gate_up, down, activation, gate_up_bias, down_bias, residual) -> N
         raise ValueError(f"down_bias must be [{hidden}]")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError("residual must have the shape and type of x")
+
+
+def wants_grad(*tensors) -> bool:
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
 def plain(param) -> bool:
@@ -87,8 +90,6 @@ class GatedFeedForwardFn(torch.autograd.Function):
 def gated_feed_forward_reference(x, gate_up, down, activation, gate_up_bias=None, down_bias=None, residual=None):
     """The block in fp32, rounded once to the type of ``x``."""
 
-    from .nn import _act_reference
-
     f = lambda t: None if t is None else t.float()  # noqa: E731
     z = torch.nn.functional.linear(x.float(), gate_up.float(), f(gate_up_bias))
     width = down.shape[1]
@@ -109,8 +110,8 @@ def gated_feed_forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tenso
     _check(x, gate_up, down, activation, gate_up_bias, down_bias, residual)
     if x.is_cuda and x.dtype == torch.bfloat16 and x.shape[0] > 0 and x.shape[1] % 8 == 0 and down.shape[1] % 8 == 0:
         args = (x, gate_up, down, gate_up_bias, down_bias, residual)
-        act = _codes()[activation]
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+        act = _CODES[activation]
+        if torch.is_grad_enabled() and wants_grad(*args):
             if plain(gate_up) and plain(down) and plain(gate_up_bias) and plain(down_bias):
                 return ext().gated_ffn_apply(*args, act, status(x.device))
             return GatedFeedForwardFn.apply(*args, act)

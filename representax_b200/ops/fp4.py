@@ -31,11 +31,12 @@ from dataclasses import dataclass
 import torch
 
 from ._ext import ext, status
-from .ffn import plain, view
+from .ffn import plain, view, wants_grad
 from .functional import _colsum_into, _GradSink
 
 FORMATS = {"mxfp4": 1, "nvfp4": 2}
 BLOCK = {"mxfp4": 32, "nvfp4": 16}
+_TYPES = frozenset((torch.bfloat16, torch.float16, torch.float32))
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
@@ -97,13 +98,12 @@ def quantize(x: torch.Tensor, fmt: str = "nvfp4", *, parts: int = 1) -> FP4Opera
     _check_format(fmt)
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"x must be a matrix with at least one column, got {tuple(x.shape)}")
-    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    if x.dtype not in _TYPES:
         raise TypeError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
     if parts < 1 or x.shape[0] % parts:
         raise ValueError(f"{x.shape[0]} rows do not split into {parts} equal parts")
-    x = x.detach()
     if not x.is_cuda:
-        return _pack_reference(x, fmt, parts)
+        return _pack_reference(x.detach(), fmt, parts)
     if x.stride(1) != 1:
         x = x.contiguous()
     data, scales, row = ext().fp4_quantize(x, parts, FORMATS[fmt])
@@ -192,7 +192,7 @@ def linear_fp4(x: torch.Tensor, weight: FP4Operand, bias: torch.Tensor | None = 
     if x.is_cuda and x.dtype == torch.bfloat16:
         if residual is not None and residual.dtype != torch.bfloat16:
             raise TypeError("residual must be bfloat16 like x")
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, bias, residual)):
+        if torch.is_grad_enabled() and wants_grad(x, bias, residual):
             if plain(bias) and x.stride(1) == 1 and (bias is None or bias.is_contiguous()):
                 return ext().fp4_linear_apply(x, weight.data, weight.scales, weight.row_scale, weight.parts,
                                               FORMATS[weight.fmt], bias, residual, status(x.device))
@@ -222,8 +222,7 @@ def gated_feed_forward_fp4(x: torch.Tensor, gate_up: FP4Operand, down: FP4Operan
         raise ValueError(f"gate_up must be [2 I, H] and down [H', I]: got {gate_up.shape} and {down.shape}")
     _check_product(x.shape[1], gate_up, gate_up_bias, None, x.shape[0])
     _check_product(down.k, down, down_bias, residual, x.shape[0])
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                           for t in (x, gate_up_bias, down_bias, residual))
+    grad = torch.is_grad_enabled() and wants_grad(x, gate_up_bias, down_bias, residual)
     if not (x.is_cuda and x.dtype == torch.bfloat16) or grad:
         h = gated_activation(linear_fp4(x, gate_up, gate_up_bias), activation)
         return linear_fp4(h, down, down_bias, residual)
