@@ -15,7 +15,7 @@ constexpr int64_t kFewTiles = 12;
 // pairs make a wave), or very few rows. Gated: up to 32 rows (two accumulators leave a ring too short beyond).
 inline bool takes(int64_t rows, int64_t cols, bool gated) {
   if (gated) return rows <= 32;
-  return rows <= 16 || (rows + 255) / 256 * ((cols + 255) / 256) <= kFewTiles;
+  return rows <= 16 || (rows + 255) / 256 * ((cols + 255) / 256) <= (rows <= 64 ? 2 : 1) * kFewTiles;
 }
 
 enum Kind : int { kBf16 = 0, kMxfp4 = 1, kNvfp4 = 2 };

@@ -50,6 +50,7 @@ constexpr int kGemmThreads = 32 * (kFirstEpi + kEpiWarps);
 // 384 * 168 that the block is launched with.
 constexpr int kIssueRegs = 64, kEpiRegs = 216;
 constexpr int kStaging = kEpiWarps * 2 * 2048;
+constexpr int kRowLd = 33;  // row of a staged tile whose output rows have any address (odd: no bank conflicts)
 
 template <int FMT>
 struct GemmShape {
@@ -60,25 +61,6 @@ struct GemmShape {
   static constexpr int kSfCols = 3 * kGroups * 4;  // TMEM columns of a stage's scales
   static_assert(256 + kGemmStages * kSfCols <= 512 && kSmem <= 232448, "does not fit");
 };
-
-// 32 consecutive outputs of row m from column n.
-__device__ __forceinline__ void store32(const GemmParams& p, int64_t m, int n, const float (&v)[32]) {
-  __nv_bfloat16* dst = p.out + m * p.ld_out + n;
-  if (p.vec && n + 32 <= p.N) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      uint4 w;
-      __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(v[8 * q + 2 * j], v[8 * q + 2 * j + 1]);
-      reinterpret_cast<uint4*>(dst)[q] = w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (n + i < p.N) dst[i] = __float2bfloat16_rn(v[i]);
-  }
-}
 
 // v += src[0..32), as far as column n + i < N.
 __device__ __forceinline__ void add32(const __nv_bfloat16* src, bool vec, int n, int N, float (&v)[32]) {
@@ -128,7 +110,7 @@ __device__ __forceinline__ void finish32(const GemmParams& p, float row_a, int64
   if (p.bias != nullptr) add32(p.bias + part0 + n, p.vec, n, p.N, v);
 }
 
-template <int FMT, bool GATED>
+template <int FMT, bool GATED, bool VEC>  // VEC: p.vec
 __global__ void __launch_bounds__(kGemmThreads, 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmSfA, const __grid_constant__ CUtensorMap tmSfB,
@@ -184,9 +166,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const int mt = u % p.m_tiles, nt = u / p.m_tiles;
       const int row0 = mt * 256 + rank * 128 + quad * 32;  // this warp's 32 rows
       uint4 next[4];  // the next chunk's residual tile, in flight
-      const bool side = !GATED && p.residual != nullptr && p.vec && row0 < p.M;
+      const bool side = VEC && !GATED && p.residual != nullptr && row0 < p.M;
       if (side && nt * kTileN + half * 128 < p.N)
         gemm::warp_fetch_tile32(p.residual, p.ld_res, row0, nt * kTileN + half * 128, p.M, p.N, lane, next);
+      // the same where rows have any address: lane = column, one load a row
+      const bool any_side = !VEC && !GATED && p.residual != nullptr && row0 < p.M;
+      const int n_end = min(p.N, nt * kTileN + half * 128 + 128);
+      __nv_bfloat16 next_any[32];
+      auto fetch_any = [&](int n) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          next_any[i] = row0 + i < p.M && n + lane < p.N
+                            ? p.residual[static_cast<int64_t>(row0 + i) * p.ld_res + n + lane]
+                            : __float2bfloat16_rn(0.f);
+      };
+      if (any_side) fetch_any(nt * kTileN + half * 128);
       bool ok = (*abort_flag == 0) && mbar_wait(tfull, local & 1, p.timeout_ns);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
@@ -211,8 +205,26 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const float row_a = FMT == kNv && live ? p.row_a[m] : 1.f;
       // 32 outputs of every row of the warp, from column n
       auto put = [&](int n, float (&v)[32], const uint4* res) {
-        if (!p.vec) {
-          if (live) store32(p, m, n, v);
+        if constexpr (!VEC) {  // rows at any address: through shared memory, a warp writes 32 columns of one row at a time
+          __nv_bfloat16* tile = reinterpret_cast<__nv_bfloat16*>(staging);
+          if (any_side) {
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) tile[i * kRowLd + lane] = next_any[i];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] += __bfloat162float(tile[lane * kRowLd + i]);
+            if (n + 32 < n_end) fetch_any(n + 32);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) tile[lane * kRowLd + i] = __float2bfloat16_rn(v[i]);
+          __syncwarp();
+          if (n + lane < p.N) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (row0 + i < p.M) p.out[static_cast<int64_t>(row0 + i) * p.ld_out + n + lane] = tile[i * kRowLd + lane];
+          }
           return;
         }
         uint8_t* buf = staging + (seq++ & 1) * 2048;
@@ -287,7 +299,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
               gemm::warp_fetch_tile32(p.residual, p.ld_res, row0, n + 32, p.M, p.N, lane, next);
             put(n, v, cur);
           } else {
-            if (p.residual != nullptr && live) add32(p.residual + m * p.ld_res + n, false, n, p.N, v);
             put(n, v, nullptr);
           }
         }
@@ -437,9 +448,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
 }
 
-template <int FMT, bool GATED>
-cudaError_t launch(const GemmMaps& maps, const GemmParams& p, int sms, int device, cudaStream_t stream) {
-  auto kern = fp4_gemm_kernel<FMT, GATED>;
+template <int FMT, bool GATED, bool VEC>
+cudaError_t launch_vec(const GemmMaps& maps, const GemmParams& p, int sms, int device, cudaStream_t stream) {
+  auto kern = fp4_gemm_kernel<FMT, GATED, VEC>;
   constexpr size_t smem = GemmShape<FMT>::kSmem;
   static bool configured[64] = {false};
   if (device < 0 || device >= 64 || !configured[device]) {
@@ -460,6 +471,12 @@ cudaError_t launch(const GemmMaps& maps, const GemmParams& p, int sms, int devic
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, maps.a, maps.b, maps.sf_a, maps.sf_b, maps.out, p);
+}
+
+template <int FMT, bool GATED>
+cudaError_t launch(const GemmMaps& maps, const GemmParams& p, int sms, int device, cudaStream_t stream) {
+  return p.vec ? launch_vec<FMT, GATED, true>(maps, p, sms, device, stream)
+               : launch_vec<FMT, GATED, false>(maps, p, sms, device, stream);
 }
 
 cudaError_t gemm(const GemmMaps& maps, const GemmParams& p, int fmt, int sms, int device, cudaStream_t stream) {

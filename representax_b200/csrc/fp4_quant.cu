@@ -72,7 +72,8 @@ struct Raw {
   static constexpr int kWords = kLane * sizeof(T) / 4;
   uint32_t w[kWords];
 
-  // Columns c.. of a row: loads of VEC bytes (0: one by one) where all exist (always, with FULL), zeros past K.
+  // Columns c.. of an aligned row: loads of VEC bytes where all exist (always, with FULL), one by one with zeros past
+  // K elsewhere.
   template <int VEC, bool FULL>
   __device__ __forceinline__ void load(const T* row, int c, int K) {
     if (VEC == 32 && (FULL || c + kLane <= K)) {
@@ -94,6 +95,25 @@ struct Raw {
 #pragma unroll
       for (int i = 0; i < kLane; ++i)
         if (c + i < K) e[i] = row[c + i];
+    }
+  }
+  // The same for a row at any address: the warp reads its piece (columns c0..) a value a lane and
+  // hands the values out through `scratch` (kPiece values of this warp).
+  __device__ __forceinline__ void load_any(const T* row, int c0, int K, T* scratch, int lane) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kLane; ++i) {
+      const int c = c0 + i * 32 + lane;
+      scratch[i * 32 + lane] = c < K ? row[c] : from_float<T>(0.f);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(scratch + lane * kLane) + i);
+      w[i] = v.x;
+      w[i + 1] = v.y;
+      w[i + 2] = v.z;
+      w[i + 3] = v.w;
     }
   }
   // Largest magnitude, in each half of the word for 16-bit types; a NaN stays one.
@@ -172,10 +192,13 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_kernel(const QuantP
   const int K = live ? p.K : 0;  // rows of the padding hold nothing
 
   Raw<T> raw[kAhead<T>];
+  __shared__ __align__(16) T scratch[VEC == 0 ? kQuantWarps * kPiece : 1];
   auto load_pieces = [&](int c, bool full) {  // c: the warp's first column
 #pragma unroll
     for (int i = 0; i < kAhead<T>; ++i) {
-      if (full)
+      if (VEC == 0)
+        raw[i].load_any(x, c + i * kPiece, K, scratch + (VEC == 0 ? warp * kPiece : 0), lane);
+      else if (full)
         raw[i].template load<VEC, true>(x, c + lane * kLane + i * kPiece, K);
       else
         raw[i].template load<VEC, false>(x, c + lane * kLane + i * kPiece, K);
@@ -326,9 +349,12 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const Dequant
   const uint8_t* q = p.q + row * p.ldq;
   const float factor = FMT == kNv ? p.row_scale[row] : 1.f;
   T* out = static_cast<T*>(p.out) + row * p.ldo;
+  __shared__ T scratch[kQuantWarps][256];
 #pragma unroll 4
-  for (int c = (warp % warps_per_row) * 256 + lane * 8; c < p.K; c += warps_per_row * 256) {
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(q + (c >> 1));
+  for (int c = (warp % warps_per_row) * 256 + lane * 8; c - lane * 8 < p.K; c += warps_per_row * 256) {  // warp-uniform
+    if (vec && c >= p.K) continue;
+    // (codes past K stay within the row of codes or count as zero)
+    const uint32_t codes = (c >> 1) < p.ldq ? *reinterpret_cast<const uint32_t*>(q + (c >> 1)) : 0u;
     const int block = c / block_of(FMT);
     const uint32_t byte = sf[static_cast<int64_t>(block >> 2) * 512 + (block & 3)];
     float scale;
@@ -343,10 +369,19 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const Dequant
     for (int j = 0; j < 8; ++j) v[j] = from_float<T>(f[j] * scale);
     if (vec && c + 8 <= p.K) {
       store8(out + c, v);
-    } else {
+    } else if (vec) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (c + j < p.K) out[c + j] = v[j];
+    } else {  // rows at any address: the warp writes its 256 values a value a lane
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) scratch[warp][lane * 8 + j] = v[j];
+      __syncwarp();
+      const int c0 = c - lane * 8;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c0 + j * 32 + lane < p.K) out[c0 + j * 32 + lane] = scratch[warp][j * 32 + lane];
     }
   }
 }
