@@ -133,7 +133,8 @@ at::Tensor bias_gradient(const at::Tensor& dy, const OptTensor& acc, at::ScalarT
 }  // namespace
 
 // bf16 products of few token rows x [T, K] with w [parts * N, K]: parts 1: x w^T (+ bias) (+ residual);
-// parts 2 (gate, up): act(x wg^T + bg) * (x wu^T + bu). `after_producer`: the launch just before, one of this kind, wrote x.
+// parts 2 (gate, up): act(x wg^T + bg) * (x wu^T + bu). `after_producer`: the launch just before, a gated projection,
+// wrote x and nothing else that this one reads.
 void few_rows_linear(const at::Tensor& x, const at::Tensor& w, int64_t parts, int64_t act,
                      const OptTensor& bias, const OptTensor& residual, at::Tensor& out,
                      bool after_producer, const at::Tensor& status) {
@@ -284,7 +285,7 @@ std::vector<at::Tensor> gated_ffn_forward(const at::Tensor& x_in, const at::Tens
     gated_forward(x, gate_up, b1, h, c10::nullopt, c10::nullopt, act, status);
   }
   if (few_down)
-    few_rows_linear(h, down, 1, 0, b2, residual, y, few_gated, status);
+    few_rows_linear(h, down, 1, 0, b2, residual, y, true, status);
   else
     gemm_tcgen05(h, down, y, false, false, (b2.has_value() ? kBias : 0) | (residual.has_value() ? kResidual : 0), kOutBf16,
                  1.0, b2, c10::nullopt, c10::nullopt, residual, status, 0, 0, 0, 0, 0.0, c10::nullopt);

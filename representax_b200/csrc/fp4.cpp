@@ -234,6 +234,7 @@ void run_product(const Operand& a, const Operand& b, int64_t act, const OptTenso
       p.q_sf = q_out->sf;
       p.q_groups = q_out->groups();
     }
+    p.after_producer = after_producer;
     p.status = status_ptr(status);
     p.timeout_ns = kWaitBudgetNs;
   };
@@ -249,7 +250,6 @@ void run_product(const Operand& a, const Operand& b, int64_t act, const OptTenso
     p.row_x = a.row;
     p.row_w = b.row;
     p.vec = out != nullptr && aligned_rows(*out, 8);
-    p.after_producer = after_producer;
     check_launch(few::launch(a.fmt, ta, tb, p, num_sms(dev), dev, stream), "fp4 product");
     return;
   }

@@ -58,6 +58,7 @@ struct GemmParams {
   int64_t ld_q;
   uint8_t* q_sf;
   int64_t q_groups;
+  int after_producer;  // the kernel before this one in the stream lets it start early; it waits for that one's end
   int* status;
   uint64_t timeout_ns;
 };

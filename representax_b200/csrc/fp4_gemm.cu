@@ -153,6 +153,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int num_units = p.m_tiles * p.n_tiles;
+  // launched early (after_producer), this grid has come this far while the one before still ran
+  grid_launch_dependents();
+  grid_dependency_wait();
 
   if (warp >= kFirstEpi) {
     // ------------------------------------------------------------ epilogue (both CTAs)
@@ -463,13 +466,15 @@ cudaError_t launch_vec(const GemmMaps& maps, const GemmParams& p, int sms, int d
   cfg.blockDim = dim3(kGemmThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = p.after_producer ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, maps.a, maps.b, maps.sf_a, maps.sf_b, maps.out, p);
 }
 

@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   cluster_sync_all();  // both CTAs' barriers are initialised before any remote use
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  grid_launch_dependents();  // the down projection may stream its weight meanwhile
   const int k_blocks = (p.K + BK - 1) / BK;
 
   if (warp == 0) {
