@@ -72,7 +72,7 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
 }
 
 template <int KIND, int PARTS, int NT>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, NT == 128 ? 2 : 3)
     few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const Params p) {
   using S = Shape<KIND, PARTS, NT>;
   extern __shared__ uint8_t smem_raw[];
@@ -248,81 +248,101 @@ __global__ void __launch_bounds__(kThreads, 2)
   grid_dependency_wait();
   const uint32_t part_addr = smem_u32(part) + lane * 16;
   const int n = tile * 128 + lane * 4;
+  constexpr int kTok = PARTS == 1 ? 2 : 1;  // tokens of a warp at a time: their loads overlap
+  // what belongs to the columns alone
+  float col_factor[PARTS][4], bias[PARTS][4];
+#pragma unroll
+  for (int b = 0; b < PARTS; ++b) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t c = static_cast<int64_t>(b) * p.N + n + j;
+      col_factor[b][j] = KIND == kNvfp4 && n + j < p.N ? p.row_w[c] : 1.f;
+      bias[b][j] = n + j < p.N && p.bias != nullptr ? __bfloat162float(p.bias[c]) : 0.f;
+    }
+  }
   if (*abort_flag == 0) {
-    for (int tl = rank * kWarps + warp; tl < tokens; tl += splits * kWarps) {
-      const int64_t t = t0 + tl;
-      // what the epilogue reads from memory first, then the partial sums of all CTAs
-      float factor[PARTS][4], bias[PARTS][4], add[4];
+    const int step = splits * kWarps;
+    for (int first_token = rank * kWarps + warp; first_token < tokens; first_token += kTok * step) {
+      // what the epilogue reads from memory, then the partial sums of all CTAs, for every token of this round
+      float row_factor[kTok], add[kTok][4];
+      float4 in[kTok][PARTS][8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool live = n + j < p.N;
-#pragma unroll
-        for (int b = 0; b < PARTS; ++b) {
-          const int64_t c = static_cast<int64_t>(b) * p.N + n + j;
-          factor[b][j] = KIND == kNvfp4 && live ? p.row_x[t] * p.row_w[c] : 1.f;
-          bias[b][j] = live && p.bias != nullptr ? __bfloat162float(p.bias[c]) : 0.f;
-        }
-        add[j] = PARTS == 1 && live && p.residual != nullptr ? __bfloat162float(p.residual[t * p.ld_res + n + j]) : 0.f;
-      }
-      float4 in[PARTS][8];
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        if (r < splits) {
-          const uint32_t peer = mapa_shared(part_addr, static_cast<uint32_t>(r));
-#pragma unroll
-          for (int b = 0; b < PARTS; ++b) in[b][r] = ld_cluster_f4(peer + (b * NT + tl) * kPartLd * 4);
-        }
-      }
-      float v[PARTS][4];
-#pragma unroll
-      for (int b = 0; b < PARTS; ++b) {
-        v[b][0] = v[b][1] = v[b][2] = v[b][3] = 0.f;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          if (r < splits) {
-            v[b][0] += in[b][r].x;
-            v[b][1] += in[b][r].y;
-            v[b][2] += in[b][r].z;
-            v[b][3] += in[b][r].w;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[b][j] = v[b][j] * factor[b][j] + bias[b][j];
-      }
-      float y[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = PARTS == 2 ? v[1 % PARTS][j] : v[0][j] + add[j];
-      if constexpr (PARTS == 2) gated::gate(p.act, v[0], y);
-      if constexpr (PARTS == 2 && KIND == kMxfp4) {
-        if (p.q_out != nullptr) {  // eight lanes hold a block of 32
-          uint32_t top = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (n + j >= p.N) y[j] = 0.f;
-            top = max(top, __float_as_uint(y[j]) & 0x7fffffffu);
-          }
-#pragma unroll
-          for (int o = 1; o < 8; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const uint32_t byte = fp4::mx_scale_byte(top);
-          const float inv = fp4::mx_inverse(byte);
-          const float w8[8] = {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv, 0.f, 0.f, 0.f, 0.f};
-          if ((n >> 1) < p.ld_q)
-            *reinterpret_cast<uint16_t*>(p.q_out + t * p.ld_q + (n >> 1)) = static_cast<uint16_t>(fp4::pack8(w8));
-          if ((lane & 7) == 0) p.q_sf[fp4::scale_offset(t, n >> 5, p.q_groups)] = static_cast<uint8_t>(byte);
-          continue;
-        }
-      }
-      __nv_bfloat16* out = p.out + t * p.ld_out + n;
-      if (p.vec && n + 4 <= p.N) {
-        uint2 w;
-        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
-        h[0] = __floats2bfloat162_rn(y[0], y[1]);
-        h[1] = __floats2bfloat162_rn(y[2], y[3]);
-        *reinterpret_cast<uint2*>(out) = w;
-      } else {
+      for (int k = 0; k < kTok; ++k) {
+        const int tl = first_token + k * step;
+        const bool live = tl < tokens;  // warp-uniform
+        row_factor[k] = KIND == kNvfp4 && live ? p.row_x[t0 + tl] : 1.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (n + j < p.N) out[j] = __float2bfloat16_rn(y[j]);
+          add[k][j] = PARTS == 1 && live && n + j < p.N && p.residual != nullptr
+                          ? __bfloat162float(p.residual[static_cast<int64_t>(t0 + tl) * p.ld_res + n + j])
+                          : 0.f;
+        if (live) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            if (r < splits) {
+              const uint32_t peer = mapa_shared(part_addr, static_cast<uint32_t>(r));
+#pragma unroll
+              for (int b = 0; b < PARTS; ++b) in[k][b][r] = ld_cluster_f4(peer + (b * NT + tl) * kPartLd * 4);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kTok; ++k) {
+        const int tl = first_token + k * step;
+        if (tl >= tokens) break;
+        const int64_t t = t0 + tl;
+        float v[PARTS][4];
+#pragma unroll
+        for (int b = 0; b < PARTS; ++b) {
+          v[b][0] = v[b][1] = v[b][2] = v[b][3] = 0.f;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            if (r < splits) {
+              v[b][0] += in[k][b][r].x;
+              v[b][1] += in[k][b][r].y;
+              v[b][2] += in[k][b][r].z;
+              v[b][3] += in[k][b][r].w;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[b][j] = v[b][j] * (row_factor[k] * col_factor[b][j]) + bias[b][j];
+        }
+        float y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = PARTS == 2 ? v[1 % PARTS][j] : v[0][j] + add[k][j];
+        if constexpr (PARTS == 2) gated::gate(p.act, v[0], y);
+        if constexpr (PARTS == 2 && KIND == kMxfp4) {
+          if (p.q_out != nullptr) {  // eight lanes hold a block of 32
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (n + j >= p.N) y[j] = 0.f;
+              top = max(top, __float_as_uint(y[j]) & 0x7fffffffu);
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const uint32_t byte = fp4::mx_scale_byte(top);
+            const float inv = fp4::mx_inverse(byte);
+            const float w8[8] = {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv, 0.f, 0.f, 0.f, 0.f};
+            if ((n >> 1) < p.ld_q)
+              *reinterpret_cast<uint16_t*>(p.q_out + t * p.ld_q + (n >> 1)) = static_cast<uint16_t>(fp4::pack8(w8));
+            if ((lane & 7) == 0) p.q_sf[fp4::scale_offset(t, n >> 5, p.q_groups)] = static_cast<uint8_t>(byte);
+            continue;
+          }
+        }
+        __nv_bfloat16* out = p.out + t * p.ld_out + n;
+        if (p.vec && n + 4 <= p.N) {
+          uint2 w;
+          __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
+          h[0] = __floats2bfloat162_rn(y[0], y[1]);
+          h[1] = __floats2bfloat162_rn(y[2], y[3]);
+          *reinterpret_cast<uint2*>(out) = w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < p.N) out[j] = __float2bfloat16_rn(y[j]);
+        }
       }
     }
   }

@@ -8,14 +8,17 @@
 namespace rx {
 namespace few {
 
-constexpr int64_t kFewTiles = 12;
-
-// Which products run here rather than on the GEMMs' CTA pairs with their 256-row tiles. Plain: where such
-// tiles would leave most of the GPU idle, that is few of them (a pair's 256 x 256 tiles of `rows` x `cols`; 74
-// pairs make a wave), or very few rows. Gated: up to 32 rows (two accumulators leave a ring too short beyond).
-inline bool takes(int64_t rows, int64_t cols, bool gated) {
+// Which products run here rather than on the GEMMs' CTA pairs, whose 256 x 256 tiles leave most of the GPU idle
+// when there are few of them (74 pairs make a wave) while K is long. Measured on both sides, us here / there:
+//   bf16 plain  [128, 6144] x 2048 outputs 16 / 35, [512, 2816] x 1024 14 / 21, [384, 6144] x 2048 29 / 36
+//   MXFP4       [128, 6144] x 2048 10.5 / 15, [128, 1152] x 768 10.2 / 9.2, [128, 768] x 2304 12 / 6.7
+//   NVFP4       [128, 6144] x 2048 11 / 19, [256, 768] x 2304 12.9 / 9.6; one row x 12288, K 2048: 8.9 / 13
+//   bf16 gated  [32, 2048] x 2 x 6144 16 / 17, [64, 2048] 24 / 17, [64, 768] x 2 x 1152 7.0 / 9.2
+// `stages`: pipeline stages along K (64 bf16 or 256 4-bit values).
+inline bool takes(int64_t rows, int64_t cols, int64_t stages, bool gated) {
   if (gated) return rows <= 32;
-  return rows <= 16 || (rows + 255) / 256 * ((cols + 255) / 256) <= (rows <= 64 ? 2 : 1) * kFewTiles;
+  const int64_t tiles = (rows + 255) / 256 * ((cols + 255) / 256);
+  return rows <= 16 || (rows <= 64 && tiles <= 24) || (tiles <= 12 && stages >= 8);
 }
 
 enum Kind : int { kBf16 = 0, kMxfp4 = 1, kNvfp4 = 2 };
