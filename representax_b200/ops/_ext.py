@@ -30,7 +30,9 @@ class KernelTimeoutError(RuntimeError):
 
 
 # Kernels launched per binding call (used to count our own launches).
-KERNELS_PER_CALL = {"attention_backward": 3, "attention_backward_bias": 3, "grad_norm_sq": 1}
+KERNELS_PER_CALL = {"attention_backward": 3, "attention_backward_bias": 3, "grad_norm_sq": 1, "gated_ffn_forward": 2,
+                    "gated_ffn_apply": 2, "gated_ffn_backward": 4, "fp4_linear": 2, "fp4_linear_apply": 2,
+                    "fp4_linear_dgrad": 2, "fp4_ffn": 3}
 
 
 class _CountingModule:

@@ -123,7 +123,7 @@ def test_quantize_strided_rows(fmt):
 
 SIZES = [(1, 128, 256), (1, 300, 64), (1, 12288, 256), (7, 1, 32), (16, 128, 512), (17, 200, 96), (33, 33, 33), (64, 1000, 1000),
          (65, 129, 300), (128, 256, 256), (129, 3330, 40), (300, 520, 1000), (513, 2050, 384), (1000, 2048, 2048), (2000, 777, 1344),
-         (40, 64, 20000)]
+         (40, 64, 20000), (100, 300, 2500), (300, 521, 2500), (129, 64, 4111)]
 
 
 @pytest.mark.parametrize("fmt", FMTS)
