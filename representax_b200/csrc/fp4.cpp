@@ -264,9 +264,7 @@ void run_product(const Operand& a, const Operand& b, int64_t act, const OptTenso
   p.b_tiles = static_cast<int>(row_tiles(N));
   p.row_a = a.row;
   p.row_b = b.row;
-  p.vec = (out == nullptr || aligned_rows(*out)) && (!residual.has_value() || aligned_rows(*residual)) &&
-          (!bias.has_value() || (aligned_rows(*bias) && (b.parts == 1 || N % 8 == 0)));
-  p.vec_rows = b.row != nullptr && reinterpret_cast<uintptr_t>(b.row) % 16 == 0 && (b.parts == 1 || N % 4 == 0);
+  p.vec = (out == nullptr || aligned_rows(*out)) && (!residual.has_value() || aligned_rows(*residual));
   fp4::GemmMaps maps;
   maps.a = make_tmap_2d_u8(a.q, M, a.code_bytes(), a.ldq, 128);
   maps.b = tb;

@@ -52,8 +52,7 @@ struct GemmParams {
   int64_t ld_res;
   __nv_bfloat16* out;  // [M, N], or null with q_out
   int64_t ld_out;
-  int vec;             // rows of out, residual and bias are 16-byte aligned: `map_out` is valid
-  int vec_rows;        // row_b allows 16-byte loads at multiples of four columns
+  int vec;             // rows of out and residual are 16-byte aligned: `map_out` is valid
   uint8_t* q_out;      // gated MXFP4 output: codes [M, ld_q] and scales
   int64_t ld_q;
   uint8_t* q_sf;

@@ -115,16 +115,10 @@ __device__ __forceinline__ void store_tile32(const uint8_t* buf, __nv_bfloat16* 
   __syncwarp();
 }
 
-__device__ __forceinline__ void add_bias32(const __nv_bfloat16* bias, int n_base, int n, float (&v)[32]) {
-  if (n_base + 32 <= n) {
-    float b[32];
-    gemm::load_bf16x32(bias + n_base, b);
+// v[i] += lane i's `bias`: a warp fetches the biases of its columns before their accumulator is ready.
+__device__ __forceinline__ void add_bias32(float bias, float (&v)[32]) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] += b[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] += n_base + i < n ? __bfloat162float(bias[n_base + i]) : 0.f;
-  }
+  for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(0xffffffffu, bias, i);
 }
 
 // Sum over the warp's lanes (rows) of each of 32 columns; lane c returns column c's.
@@ -316,6 +310,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           next_e = p.exps[t * 32 + lane];
         }
       }
+      float bias_g[2] = {}, bias_u[2] = {};
+      if constexpr (!kDz) {
+        static_assert(kChunks == 2, "two chunks of 32 columns a warp");
+        if (p.bias != nullptr) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int n = n0 + (chunk0 + c) * 32 + lane;
+            if (n < p.N) {
+              bias_g[c] = __bfloat162float(p.bias[n]);
+              bias_u[c] = __bfloat162float(p.bias[p.N + n]);
+            }
+          }
+        }
+      }
       bool ok = (*abort_flag == 0) && mbar_wait(&tfull[acc], (local >> 1) & 1, p.timeout_ns);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
@@ -379,8 +387,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             v[i] = __uint_as_float(ru[i]);
           }
           if (p.bias != nullptr) {
-            add_bias32(p.bias, n, p.N, g);
-            add_bias32(p.bias + p.N, n, p.N, v);
+            add_bias32(c == chunk0 ? bias_g[0] : bias_g[1], g);
+            add_bias32(c == chunk0 ? bias_u[0] : bias_u[1], v);
           }
           if (n + 32 > p.N) {  // columns past the end (the gate side holds up rows there) count as zero
 #pragma unroll
@@ -390,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if constexpr (kSave) {
             float b[32];
             float top_a = 0.f, top_b = 0.f;
-gate_and_keep(p.act, g, v, b);
+            gate_and_keep(p.act, g, v, b);
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               top_a = fmaxf(top_a, fabsf(g[i]));
