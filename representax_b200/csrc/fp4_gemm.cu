@@ -50,7 +50,7 @@ constexpr int kGemmThreads = 32 * (kFirstEpi + kEpiWarps);
 // 384 * 168 that the block is launched with.
 constexpr int kIssueRegs = 64, kEpiRegs = 216;
 constexpr int kStaging = kEpiWarps * 2 * 2048;
-constexpr int kRowLd = 33;  // row of a staged tile whose output rows have any address (odd: no bank conflicts)
+constexpr int kRowLd = 34;  // row of a staged tile whose output rows have any address (17 words: no bank conflicts)
 
 template <int FMT>
 struct GemmShape {
@@ -144,13 +144,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       // the same where rows have any address: lane = column, one load a row
       const bool any_side = !VEC && !GATED && p.residual != nullptr && row0 < p.M;
       const int n_end = min(p.N, nt * kTileN + half * 128 + 128);
+      const bool rows_full = row0 + 32 <= p.M;
       __nv_bfloat16 next_any[32];
       auto fetch_any = [&](int n) {
+        const __nv_bfloat16* src = p.residual + static_cast<int64_t>(row0) * p.ld_res + n + lane;
+        if (rows_full && n + 32 <= p.N) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          next_any[i] = row0 + i < p.M && n + lane < p.N
-                            ? p.residual[static_cast<int64_t>(row0 + i) * p.ld_res + n + lane]
-                            : __float2bfloat16_rn(0.f);
+          for (int i = 0; i < 32; ++i, src += p.ld_res) next_any[i] = *src;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i, src += p.ld_res)
+            next_any[i] = row0 + i < p.M && n + lane < p.N ? *src : __float2bfloat16_rn(0.f);
+        }
       };
       if (any_side) fetch_any(nt * kTileN + half * 128);
       // row factors and biases of the four chunks of 32 columns, lane = column (gated: two of gate, two of up)
@@ -191,23 +196,35 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       auto put = [&](int n, float (&v)[32], const uint4* res) {
         if constexpr (!VEC) {  // rows at any address: through shared memory, a warp writes 32 columns of one row at a time
           __nv_bfloat16* tile = reinterpret_cast<__nv_bfloat16*>(staging);
+          uint32_t* row = reinterpret_cast<uint32_t*>(tile + lane * kRowLd);
           if (any_side) {
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < 32; ++i) tile[i * kRowLd + lane] = next_any[i];
             __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += __bfloat162float(tile[lane * kRowLd + i]);
+            for (int i = 0; i < 16; ++i) {
+              const uint32_t w = row[i];
+              v[2 * i] += __uint_as_float(w << 16);
+              v[2 * i + 1] += __uint_as_float(w & 0xffff0000u);
+            }
             if (n + 32 < n_end) fetch_any(n + 32);
           }
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) tile[lane * kRowLd + i] = __float2bfloat16_rn(v[i]);
+          for (int i = 0; i < 16; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            row[i] = *reinterpret_cast<const uint32_t*>(&h);
+          }
           __syncwarp();
-          if (n + lane < p.N) {
+          __nv_bfloat16* dst = p.out + static_cast<int64_t>(row0) * p.ld_out + n + lane;
+          if (rows_full && n + 32 <= p.N) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (row0 + i < p.M) p.out[static_cast<int64_t>(row0 + i) * p.ld_out + n + lane] = tile[i * kRowLd + lane];
+            for (int i = 0; i < 32; ++i, dst += p.ld_out) *dst = tile[i * kRowLd + lane];
+          } else if (n + lane < p.N) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i, dst += p.ld_out)
+              if (row0 + i < p.M) *dst = tile[i * kRowLd + lane];
           }
           return;
         }

@@ -97,23 +97,58 @@ struct Raw {
         if (c + i < K) e[i] = row[c + i];
     }
   }
-  // The same for a row at any address: the warp reads its piece (columns c0..) a value a lane and
-  // hands the values out through `scratch` (kPiece values of this warp).
-  __device__ __forceinline__ void load_any(const T* row, int c0, int K, T* scratch, int lane) {
+  // The same for a row at any address: the warp reads its piece (columns c0.., c0 < K) in 16-byte pieces from the
+  // boundary before it, those that cross the row's ends a value at a time, and hands the values out through
+  // `scratch` (kScratch words of this warp; a word of padding after eight, so that lanes do not meet in a bank).
+  static constexpr int kScratch = (kPiece * static_cast<int>(sizeof(T)) / 4 + 4) / 8 * 9 + 8;
+  __device__ __forceinline__ void load_any(const T* row, int c0, int K, uint32_t* scratch, int lane) {
+    constexpr int kSize = sizeof(T), kVecs = kPiece * kSize / 16;
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row + c0) & 15);  // bytes of the first vector before the piece
+    const char* base = reinterpret_cast<const char*>(row + c0) - off;
+    const int64_t end = off + static_cast<int64_t>(K - c0) * kSize;  // of the row
+    auto fetch = [&](int b) {                               // bytes b.. of the vectors
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if ((b >= off || c0 > 0) && b + 16 <= end) {
+        v = ldg_v4_issue(base + b);
+      } else {
+        T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+        for (int i = 0; i < 16 / kSize; ++i) {
+          const int at = b + i * kSize;
+          if (at >= off && at < end) e[i] = *reinterpret_cast<const T*>(base + at);
+        }
+      }
+      return v;
+    };
+    auto put = [&](int word, const uint4& v) {  // word: a multiple of four
+      uint32_t* dst = scratch + word + (word >> 3);
+      dst[0] = v.x;
+      dst[1] = v.y;
+      dst[2] = v.z;
+      dst[3] = v.w;
+    };
+    uint4 v[kVecs / 32];
+#pragma unroll
+    for (int i = 0; i < kVecs / 32; ++i) v[i] = fetch(16 * (lane + 32 * i));
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < kLane; ++i) {
-      const int c = c0 + i * 32 + lane;
-      scratch[i * 32 + lane] = c < K ? row[c] : from_float<T>(0.f);
-    }
+    for (int i = 0; i < kVecs / 32; ++i) put(4 * (lane + 32 * i), v[i]);
+    if (lane == 0 && off > 0) put(4 * kVecs, fetch(16 * kVecs));
     __syncwarp();
+    const int first = (off >> 2) + lane * kWords;
+    auto word = [&](int i) { return scratch[first + i + ((first + i) >> 3)]; };
+    if constexpr (kSize == 4) {
 #pragma unroll
-    for (int i = 0; i < kWords; i += 4) {
-      const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(scratch + lane * kLane) + i);
-      w[i] = v.x;
-      w[i + 1] = v.y;
-      w[i + 2] = v.z;
-      w[i + 3] = v.w;
+      for (int i = 0; i < kWords; ++i) w[i] = word(i);
+    } else {
+      const int shift = (off & 2) * 8;
+      uint32_t low = word(0);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        const uint32_t high = word(i + 1);
+        w[i] = __funnelshift_r(low, high, shift);
+        low = high;
+      }
     }
   }
   // Largest magnitude, in each half of the word for 16-bit types; a NaN stays one.
@@ -247,7 +282,7 @@ __global__ void __launch_bounds__(kQuantThreads, VEC != 0 && AHEAD * sizeof(T) =
   const bool kept = FMT == kNv && stride >= extent;  // the maximum's pass leaves the whole row in registers
 
   Raw<T> raw[AHEAD];
-  __shared__ __align__(16) T scratch[VEC == 0 ? kQuantWarps * kPiece : 1];
+  __shared__ uint32_t scratch[VEC == 0 ? kQuantWarps * Raw<T>::kScratch : 1];
   // The pieces from column c on; those past K are zeros. At most one piece of a row ends inside.
   auto load_pieces = [&](int c) {
     const int full = min(max(K - c, 0) / kPiece, AHEAD);
@@ -256,7 +291,7 @@ __global__ void __launch_bounds__(kQuantThreads, VEC != 0 && AHEAD * sizeof(T) =
       if (VEC != 0 && i < full)
         raw[i].template load<VEC, true>(x, c + i * kPiece + lane * kLane, K);
       else if (VEC == 0 && c + i * kPiece < K)
-        raw[i].load_any(x, c + i * kPiece, K, scratch + (VEC == 0 ? warp * kPiece : 0), lane);
+        raw[i].load_any(x, c + i * kPiece, K, scratch + (VEC == 0 ? warp * Raw<T>::kScratch : 0), lane);
       else
         raw[i].clear();
     }

@@ -338,3 +338,16 @@ def test_model_with_4bit_weights(fmt):
     again.load_state_dict(state)
     with torch.no_grad():
         assert torch.equal(again(emb, seg, pos), a)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("c", [1, 9, 511, 1029, 2600])
+def test_quantize_rows_at_any_address(fmt, dtype, c):
+    from representax_b200.ops.fp4 import quantize
+
+    flat = _randn(4 * (c + 9) + 16, seed=c, dtype=dtype)
+    for offset in range(9):
+        for pitch in (c, c + 9):
+            x = flat[offset:offset + 3 * pitch + c].as_strided((4, c), (pitch, 1))
+            _same(quantize(x, fmt), quantize(x.contiguous().cpu(), fmt))
