@@ -32,6 +32,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "fp4.cuh"
@@ -258,8 +259,8 @@ __device__ __forceinline__ float quotient(float a, float s, float inv) {
 // The warps of a row (blockDim.x / 32, up to 8) take spans of AHEAD pieces in turn; in MXFP4, where spans do not
 // depend on one another, blockIdx.y goes over them. All scale bytes of the row tiles are written, those of the
 // padding included. Occupancy: the registers of four 16-bit pieces let three CTAs fit; with four CTAs they spill
-// ([12283, 2048] fp32 NVFP4 27.3 instead of 26.4 us). Rows at any address are read through shared memory and
-// want four (59.5 instead of 66.5 us at [8191, 5001] fp16).
+// ([12283, 2048] fp32 NVFP4 27.3 instead of 26.4 us). Rows at any address pass through shared memory and
+// take at most two pieces and four CTAs ([8191, 5001] fp16 NVFP4: 46 us, four pieces 53, four and three CTAs 55).
 template <typename T, int FMT, int VEC, int AHEAD>
 __global__ void __launch_bounds__(kQuantThreads, VEC != 0 && AHEAD * sizeof(T) == 8 ? 3 : 4) quantize_kernel(const QuantParams p) {
   __shared__ uint32_t tops[kQuantWarps];
@@ -407,7 +408,7 @@ cudaError_t launch_quantize(const QuantParams& p, cudaStream_t stream) {
 template <typename T, int FMT, int VEC>
 cudaError_t launch_ahead(int ahead, const QuantParams& p, cudaStream_t stream) {
   if (ahead == 1) return launch_quantize<T, FMT, VEC, 1>(p, stream);
-  if constexpr (sizeof(T) == 2)
+  if constexpr (sizeof(T) == 2 && VEC != 0)
     if (ahead > 2) return launch_quantize<T, FMT, VEC, 4>(p, stream);
   return launch_quantize<T, FMT, VEC, 2>(p, stream);
 }
@@ -426,7 +427,7 @@ cudaError_t quantize_typed(const QuantParams& p, cudaStream_t stream) {
   const int ahead = pieces == 1 || (few && pieces <= kQuantWarps) ? 1 : pieces == 2 || (few && pieces <= 2 * kQuantWarps) ? 2 : 4;
   if (aligned(32)) return launch_ahead<T, FMT, 32>(ahead, p, stream);
   if (aligned(16)) return launch_ahead<T, FMT, 16>(ahead, p, stream);
-  return launch_quantize<T, FMT, 0, 4 / sizeof(T)>(p, stream);
+  return launch_ahead<T, FMT, 0>(std::min(ahead, 2), p, stream);
 }
 
 cudaError_t quantize(const QuantParams& p, int fmt, int type, cudaStream_t stream) {
