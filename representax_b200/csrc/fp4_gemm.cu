@@ -28,8 +28,8 @@
 // against 110 and 121 us with the warp-uniform loop. What bounds it now is the
 // L2: without an epilogue the loads run at 12 TB/s over all SMs, 5.4 PFLOP/s;
 // the epilogue's stores come on top. K 6144, 8192 x 2048 outputs + residual:
-// 49 us MXFP4 (4.2 PFLOP/s), 58 us NVFP4; gated, K 2048, 8192 x 6144 outputs as
-// MXFP4 codes: 97 us (4.3 PFLOP/s).
+// 53 us MXFP4 (3.9 PFLOP/s), 54 us NVFP4; gated, K 2048, 8192 x 6144 outputs as
+// MXFP4 codes: 95 us (4.3 PFLOP/s), NVFP4 with bf16 outputs 102 us.
 #include "fp4.h"
 
 #include <algorithm>
