@@ -26,7 +26,7 @@
 //    IBM RISC System/6000 processor", 1990): the correctly rounded quotient
 //    in three operations, so ties fall as the definition says.
 // [8192, 6144] bf16: MXFP4 26 us (127 MB, 4.9 TB/s), NVFP4 32 us (4.1 TB/s, 41 us when one warp a row read it twice);
-// [12283, 2048] fp32: 23 us (5.0 TB/s) and 26 us (33 us); decoding that to fp32 24 us (114 MB, 4.7 TB/s).
+// [12283, 2048] fp32: 23 us (5.0 TB/s) and 26 us (33 us); decoding that to fp32 23 us (114 MB, 4.9 TB/s).
 #include "fp4.h"
 
 #include <cuda_fp16.h>
@@ -453,9 +453,10 @@ __device__ __forceinline__ void store8(T* dst, const T (&v)[8]) {
 
 // A lane decodes eight consecutive values at a time, a warp 256. Rows as in the quantiser.
 template <typename T, int FMT>
-__global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const DequantParams p, int warps_per_row, bool vec) {
-  const int warp = warp_id(), lane = lane_id();
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kQuantWarps / warps_per_row) + warp / warps_per_row;
+__global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const DequantParams p, bool vec) {
+  const int place = threadIdx.x >> 5, lane = threadIdx.x & 31, warps_per_row = blockDim.x >> 5;
+  const int warp = threadIdx.y * warps_per_row + place;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   if (row >= p.parts * p.rows) return;
   const int64_t part = p.parts == 1 ? 0 : row / p.rows;
   const uint8_t* sf = p.sf + scale_offset(part * ((p.rows + 127) / 128 * 128) + row - part * p.rows, 0, p.groups);
@@ -464,7 +465,7 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const Dequant
   T* out = static_cast<T*>(p.out) + row * p.ldo;
   __shared__ T scratch[kQuantWarps][256];
 #pragma unroll 4
-  for (int c = (warp % warps_per_row) * 256 + lane * 8; c - lane * 8 < p.K; c += warps_per_row * 256) {  // warp-uniform
+  for (int c = place * 256 + lane * 8; c - lane * 8 < p.K; c += warps_per_row * 256) {  // warp-uniform
     if (vec && c >= p.K) continue;
     // (codes past K stay within the row of codes or count as zero)
     const uint32_t codes = (c >> 1) < p.ldq ? *reinterpret_cast<const uint32_t*>(q + (c >> 1)) : 0u;
@@ -504,12 +505,17 @@ cudaError_t dequantize_typed(const DequantParams& p, int fmt, cudaStream_t strea
   constexpr int kAlign = 8 * sizeof(T);
   const bool vec = reinterpret_cast<uintptr_t>(p.out) % kAlign == 0 && p.ldo % 8 == 0;
   const int64_t rows = p.parts * p.rows;
-  const int wpr = row_warps(rows, (p.K + 255) / 256);
-  const unsigned grid = static_cast<unsigned>((rows * wpr + kQuantWarps - 1) / kQuantWarps);
+  // four pieces of 256 values a warp, fewer while that leaves SMs with less than 32 warps ([2048, 6144] bf16 MXFP4: a whole row a
+  // warp 13.0 us, four pieces 10.3; [12288, 2048] 18.6 and 16.4, one piece 20.2)
+  const int pieces = (p.K + 255) / 256;
+  int wpr = std::min(kQuantWarps, (pieces + 3) / 4);
+  if (rows * wpr < 148 * 32) wpr = std::min(kQuantWarps, pieces);
+  const dim3 threads(32 * wpr, kQuantWarps / wpr);
+  const unsigned grid = static_cast<unsigned>((rows + threads.y - 1) / threads.y);
   if (fmt == kMx)
-    dequantize_kernel<T, kMx><<<grid, kQuantThreads, 0, stream>>>(p, wpr, vec);
+    dequantize_kernel<T, kMx><<<grid, threads, 0, stream>>>(p, vec);
   else
-    dequantize_kernel<T, kNv><<<grid, kQuantThreads, 0, stream>>>(p, wpr, vec);
+    dequantize_kernel<T, kNv><<<grid, threads, 0, stream>>>(p, vec);
   return cudaGetLastError();
 }
 
