@@ -147,6 +147,8 @@ def _normal(shape, std, g):
 
 
 class CLIPEncoder(nn.Module):
+    packed_linears = {"text_projection": 1, "visual_projection": 1}
+
     def __init__(self, config: CLIPConfig, *, seed: int = 0, model_id: str = "representax/clip",
                  revision: str = "random-init", compute_dtype: torch.dtype = torch.float32) -> None:
         super().__init__()

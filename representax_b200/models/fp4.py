@@ -1,12 +1,17 @@
 """Frozen linear weights held in microscaled 4-bit floating point.
 
-``quantize_linears_fp4`` swaps the 2-D linear weights of an encoder for
+``quantize_linears_fp4`` swaps linear weights of an encoder for
 :class:`FP4Weight` submodules under the same attribute names; the packed-row
 linear and feed-forward helpers of ``ops.nn`` dispatch on them, so the encoder
 then embeds with 4-bit products (``ops.fp4``). It is a serving transform: the
-weights are frozen and no longer export; save or export the model first. Fused
-gate / up projections are quantised in their two parts, which the gated
-feed-forward kernel needs.
+weights are frozen and no longer export; save or export the model first.
+
+Only weights that reach nothing but those helpers can be swapped. A module says
+which by a class attribute ``packed_linears``: attribute name -> parts of its
+rows (2 for a fused gate / up projection, whose halves the gated feed-forward
+kernel needs apart). The Qwen3, Qwen3-VL, Qwen2.5-Omni, ModernVBERT and CLIP layers have one.
+Everything else (embeddings, lookup tables, patch projections, heads, LoRA
+factors, the BERT and MPNet blocks) keeps its weights; a model without such layers is refused.
 
 Parity: the weight-swapping entry of src/representax/models/adapters.py:30-267
 (``apply_quantized_lora``), for a format that the reference does not have.
@@ -20,11 +25,6 @@ import torch
 from torch import nn
 
 from representax_b200.ops.fp4 import BLOCK, FP4Operand, dequantize, quantize
-
-# Attribute names of fused [gate; up] weights.
-_GATED = re.compile(r"(^|\.)(gate_up|gate_up_w|Wi)$")
-# 2-D parameters that are not linear weights of the towers.
-_SKIP = re.compile(r"embed|embeddings\.|\.word$|^word$|position|pos_embed|class_embedding|patch_w$|connector")
 
 
 class FP4Weight(nn.Module):
@@ -59,22 +59,30 @@ class FP4Weight(nn.Module):
 
 
 def quantize_linears_fp4(model: nn.Module, *, fmt: str = "nvfp4", target_pattern: str = ".*") -> nn.Module:
-    """Swap every matching 2-D linear weight of ``model`` for an :class:`FP4Weight` and freeze the rest."""
+    """Swap every matching linear weight of ``model``'s packed-row layers for an :class:`FP4Weight` and freeze the rest.
 
+    The model is changed only after every weight has been quantised, so a
+    refusal leaves it as it was."""
+
+    if fmt not in BLOCK:
+        raise ValueError(f"fmt must be one of {sorted(BLOCK)}, got {fmt!r}")
     pattern = re.compile(target_pattern)
-    targets = []
+    able = []
     for mod_name, module in model.named_modules():
-        for attr, p in list(module._parameters.items()):
-            full = f"{mod_name}.{attr}" if mod_name else attr
-            if p is not None and p.ndim == 2 and not _SKIP.search(full) and pattern.search(full):
-                targets.append((module, attr, full))
+        for attr, parts in getattr(type(module), "packed_linears", {}).items():
+            if module._parameters.get(attr) is not None:
+                able.append((module, attr, f"{mod_name}.{attr}" if mod_name else attr, parts))
+    if not able:
+        raise ValueError(f"{type(model).__name__} has no linear weights that run on packed rows in 4 bits")
+    targets = [t for t in able if pattern.search(t[2])]
     if not targets:
         raise ValueError(f"no linear weights match target_pattern {target_pattern!r}")
+    swapped = [FP4Weight(module._parameters[attr], fmt=fmt, parts=parts) for module, attr, _, parts in targets]
     for p in model.parameters():
         p.requires_grad_(False)
-    for module, attr, full in targets:
-        weight = module._parameters.pop(attr)
-        module.add_module(attr, FP4Weight(weight, fmt=fmt, parts=2 if _GATED.search(full) else 1))
+    for (module, attr, _, _), weight in zip(targets, swapped):
+        del module._parameters[attr]
+        module.add_module(attr, weight)
     return model
 
 

@@ -44,6 +44,8 @@ def _embed(ids: torch.Tensor, table: torch.Tensor, dtype: torch.dtype) -> torch.
 
 # --------------------------------------------------------------- text tower
 class ModernBertLayer(nn.Module):
+    packed_linears = {"Wqkv": 1, "Wo": 1, "Wi": 2, "mlp_Wo": 1}
+
     def __init__(self, cfg: ModernVBERTTextConfig, index: int, g: torch.Generator) -> None:
         super().__init__()
         h, i, std = cfg.hidden_size, cfg.intermediate_size, cfg.initializer_range
@@ -155,6 +157,8 @@ def _unpack(h: torch.Tensor, mask: torch.Tensor) -> torch.Tensor:
 # ------------------------------------------------------------- vision tower
 class VisionLayer(nn.Module):
     """Pre-LN transformer block (fused q/k/v) used by the SigLIP and CLIP towers."""
+
+    packed_linears = {"qkv_w": 1, "out_w": 1, "fc1_w": 1, "fc2_w": 1}
 
     def __init__(self, hidden: int, inter: int, g: torch.Generator, std: float = 0.02) -> None:
         super().__init__()

@@ -214,6 +214,8 @@ def _normal(shape, std, g):
 
 # ------------------------------------------------------------------ vision
 class _OmniVisionBlock(nn.Module):
+    packed_linears = {"qkv_w": 1, "proj_w": 1, "gate_up_w": 2, "down_w": 1}
+
     def __init__(self, cfg: OmniVisionConfig, g) -> None:
         super().__init__()
         h, i = cfg.hidden_size, cfg.intermediate_size
@@ -233,6 +235,8 @@ class _OmniVisionBlock(nn.Module):
 
 
 class OmniVisionTower(nn.Module):
+    packed_linears = {"fc1_w": 1, "fc2_w": 1}
+
     def __init__(self, cfg: OmniVisionConfig, g) -> None:
         super().__init__()
         self.config = cfg
@@ -281,6 +285,8 @@ def _conv1d(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, stride: i
 
 
 class OmniAudioTower(nn.Module):
+    packed_linears = {"proj_w": 1}
+
     def __init__(self, cfg: OmniAudioConfig, g) -> None:
         super().__init__()
         self.config = cfg

@@ -93,6 +93,8 @@ def _normal(shape, std, g):
 
 
 class Qwen3DecoderLayer(nn.Module):
+    packed_linears = {"qkv": 1, "o_proj": 1, "gate_up": 2, "down": 1}
+
     def __init__(self, cfg: Qwen3TextConfig, g: torch.Generator) -> None:
         super().__init__()
         h, d, std = cfg.hidden_size, cfg.head_dimension, cfg.initializer_range

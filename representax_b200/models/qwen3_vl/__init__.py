@@ -267,6 +267,8 @@ def _normal(shape, std, g):
 
 
 class _Merger(nn.Module):
+    packed_linears = {"fc1_w": 1, "fc2_w": 1}
+
     def __init__(self, cfg: Qwen3VLVisionConfig, postshuffle: bool, g) -> None:
         super().__init__()
         wide = cfg.hidden_size * cfg.spatial_merge_size ** 2
@@ -286,6 +288,8 @@ class _Merger(nn.Module):
 
 
 class _VisionBlock(nn.Module):
+    packed_linears = {"qkv_w": 1, "proj_w": 1, "fc1_w": 1, "fc2_w": 1}
+
     def __init__(self, cfg: Qwen3VLVisionConfig, g) -> None:
         super().__init__()
         h, i = cfg.hidden_size, cfg.intermediate_size
