@@ -63,6 +63,12 @@ def view(param):
     return param if plain(param) else compute_view(param)
 
 
+def kernel_widths(hidden: int, width: int) -> bool:
+    """Whether the kernels take blocks of these sizes (rows that the tensor maps can read: multiples of 16 bytes)."""
+
+    return hidden % 8 == 0 and width % 8 == 0
+
+
 class GatedFeedForwardFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_up, down, gate_up_bias, down_bias, residual, act):
@@ -108,7 +114,7 @@ def gated_feed_forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tenso
     with a ``main_grad`` accumulate into it in fp32)."""
 
     _check(x, gate_up, down, activation, gate_up_bias, down_bias, residual)
-    if x.is_cuda and x.dtype == torch.bfloat16 and x.shape[0] > 0 and x.shape[1] % 8 == 0 and down.shape[1] % 8 == 0:
+    if x.is_cuda and x.dtype == torch.bfloat16 and x.shape[0] > 0 and kernel_widths(x.shape[1], down.shape[1]):
         args = (x, gate_up, down, gate_up_bias, down_bias, residual)
         act = _CODES[activation]
         if torch.is_grad_enabled() and wants_grad(*args):
@@ -120,4 +126,4 @@ def gated_feed_forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tenso
     return gated_feed_forward_reference(x, gate_up, down, activation, gate_up_bias, down_bias, residual)
 
 
-__all__ = ["GatedFeedForwardFn", "gated_feed_forward", "gated_feed_forward_reference"]
+__all__ = ["GatedFeedForwardFn", "gated_feed_forward", "gated_feed_forward_reference", "kernel_widths"]

@@ -498,7 +498,9 @@ def fused_feed_forward(enabled: bool = True) -> Iterator[None]:
     """Run the gated feed-forward blocks of models called inside as the fused kernels of ``ops.ffn``.
 
     Off by default: the separate layers round the projections to bf16 where the
-    fused block keeps them in fp32, so results differ in the last bits."""
+    fused block keeps them in fp32, so results differ in the last bits. Like the
+    precision policy this belongs to the calling context: a thread started inside
+    has to enter it itself."""
 
     token = _FUSED_FEED_FORWARD.set(enabled)
     try:
@@ -512,7 +514,8 @@ def gated_mlp(x: torch.Tensor, gate_up, down, name: str, gate_up_bias: torch.Ten
     """A layer's gated feed-forward block, ``(act(g) * u) down^T`` with ``[g u] = x gate_up^T``.
 
     4-bit weights run the 4-bit block of ``ops.fp4``; plain weights the separate
-    layers, or the fused kernels inside :func:`fused_feed_forward` (not under an fp8 policy)."""
+    layers, or the fused kernels inside :func:`fused_feed_forward` (not under an
+    fp8 policy, nor at widths that are not multiples of 8)."""
 
     from representax_b200.models.fp4 import FP4Weight
 
@@ -523,10 +526,11 @@ def gated_mlp(x: torch.Tensor, gate_up, down, name: str, gate_up_bias: torch.Ten
                                       down_bias=down_bias, residual=residual)
     if (_FUSED_FEED_FORWARD.get() and isinstance(gate_up, torch.Tensor) and isinstance(down, torch.Tensor)
             and native(x) and not _fp8_matrices()):
-        from .ffn import gated_feed_forward
+        from .ffn import gated_feed_forward, kernel_widths
 
-        return gated_feed_forward(x, gate_up, down, activation=name, gate_up_bias=gate_up_bias, down_bias=down_bias,
-                                  residual=residual)
+        if kernel_widths(x.shape[1], down.shape[1]):  # else the fp32 statement: slower than the separate layers
+            return gated_feed_forward(x, gate_up, down, activation=name, gate_up_bias=gate_up_bias, down_bias=down_bias,
+                                      residual=residual)
     return linear(gated_activation(linear(x, gate_up, gate_up_bias), name), down, down_bias, residual=residual)
 
 
