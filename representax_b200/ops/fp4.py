@@ -18,7 +18,8 @@ A layer's weight is quantised once (:func:`quantize`, or
 ``models.fp4.FP4Weight`` inside a model); its activations are quantised inside
 every call. bf16 CUDA rows run the kernels, anything else the PyTorch statement.
 Weights are frozen: the backward pass gives the gradients of the input
-(``dx = dy Q(W)``, the quantiser counted as the identity), bias and residual.
+(``dx = dy Q(W)``, the quantiser counted as the identity), bias and residual. A
+forward pass gives the same values whether or not a gradient is asked for.
 
 Parity: no counterpart in the reference; the 4-bit sibling of its fp8 linear
 (src/representax/precision.py:127-221).
@@ -156,6 +157,19 @@ def _linear(x, w: FP4Operand, bias, residual):
                             status(x.device))
 
 
+def _dgrad(dy, w: FP4Operand):
+    return ext().fp4_linear_dgrad(dy, w.data, w.scales, w.row_scale, w.parts, w.k, FORMATS[w.fmt], status(dy.device))
+
+
+def _bias_gradient(dy, bias):
+    sink = _GradSink(bias)
+    if dy.shape[0] and dy.shape[1] % 8 == 0 and dy.is_contiguous() and dy.data_ptr() % 16 == 0:
+        _colsum_into(dy, sink)
+    else:
+        sink.buffer().add_(dy.float().sum(0))
+    return sink.result()
+
+
 class LinearFP4Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual):
@@ -169,14 +183,9 @@ class LinearFP4Fn(torch.autograd.Function):
         w = ctx.weight
         dx = db = None
         if ctx.needs_input_grad[0]:
-            dx = ext().fp4_linear_dgrad(dy, w.data, w.scales, w.row_scale, w.parts, w.k, FORMATS[w.fmt], status(dy.device))
+            dx = _dgrad(dy, w)
         if ctx.needs_input_grad[2]:
-            sink = _GradSink(bias)
-            if dy.shape[0] and dy.shape[1] % 8 == 0 and dy.is_contiguous() and dy.data_ptr() % 16 == 0:
-                _colsum_into(dy, sink)
-            else:
-                sink.buffer().add_(dy.float().sum(0))
-            db = sink.result()
+            db = _bias_gradient(dy, bias)
         return dx, None, db, dy if ctx.needs_input_grad[3] else None
 
 
@@ -201,6 +210,48 @@ def linear_fp4(x: torch.Tensor, weight: FP4Operand, bias: torch.Tensor | None = 
     return linear_fp4_reference(x, weight, bias, residual)
 
 
+def _feed_forward(x, gate_up: FP4Operand, down: FP4Operand, activation, gate_up_bias, down_bias, residual):
+    from .nn import ACT_CODES
+
+    bias = lambda t: None if t is None else view(t).contiguous()  # noqa: E731
+    return ext().fp4_ffn(x if x.stride(1) == 1 else x.contiguous(), gate_up.data, gate_up.scales, gate_up.row_scale,
+                         FORMATS[gate_up.fmt], down.data, down.scales, down.row_scale, FORMATS[down.fmt],
+                         ACT_CODES[activation], bias(gate_up_bias), bias(down_bias), residual, status(x.device))
+
+
+class GatedFeedForwardFP4Fn(torch.autograd.Function):
+    """The block's own forward, so that a value does not depend on whether its gradient is asked for. The backward
+    runs the first product once more (z in bf16) instead of keeping [T, 2 I] values of it."""
+
+    @staticmethod
+    def forward(ctx, x, gate_up, down, activation, gate_up_bias, down_bias, residual):
+        ctx.weights, ctx.activation = (gate_up, down), activation
+        ctx.save_for_backward(x, gate_up_bias, down_bias)
+        return _feed_forward(x, gate_up, down, activation, gate_up_bias, down_bias, residual)
+
+    @staticmethod
+    def backward(ctx, dy):
+        from .nn import gated_activation
+
+        x, gate_up_bias, down_bias = ctx.saved_tensors
+        gate_up, down = ctx.weights
+        need = ctx.needs_input_grad
+        dx = db1 = db2 = None
+        if need[0] or need[4]:
+            if dy.shape[0]:
+                z = _linear(x, gate_up, gate_up_bias, None).requires_grad_()
+                with torch.enable_grad():
+                    h = gated_activation(z, ctx.activation)
+                (dz,) = torch.autograd.grad(h, z, _dgrad(dy, down))
+            else:
+                dz = dy.new_zeros(0, gate_up.rows)
+            dx = _dgrad(dz, gate_up) if need[0] else None
+            db1 = _bias_gradient(dz, gate_up_bias) if need[4] else None
+        if need[5]:
+            db2 = _bias_gradient(dy, down_bias)
+        return dx, None, None, None, db1, db2, dy if need[6] else None
+
+
 def gated_feed_forward_fp4(x: torch.Tensor, gate_up: FP4Operand, down: FP4Operand, *, activation: str,
                            gate_up_bias: torch.Tensor | None = None, down_bias: torch.Tensor | None = None,
                            residual: torch.Tensor | None = None) -> torch.Tensor:
@@ -209,10 +260,10 @@ def gated_feed_forward_fp4(x: torch.Tensor, gate_up: FP4Operand, down: FP4Operan
     ``h = act(Q(x) Q(Wg)^T + bg) * (Q(x) Q(Wu)^T + bu)``, ``y = Q(h) Q(Wd)^T + bd
     (+ residual)``; ``gate_up`` is quantised with ``parts=2``. In MXFP4 the first
     product's kernel quantises its fp32 results itself (h is never written in 16
-    bits); in NVFP4, whose row factor needs the whole row, h passes through bf16.
-    Where a gradient is asked for, the block runs as separate layers."""
+    bits); in NVFP4, whose row factor needs the whole row, h passes through the type of x.
+    Gradients of x, the biases and the residual (both quantisers counted as the identity)."""
 
-    from .nn import ACT_CODES, gated_activation
+    from .nn import ACT_CODES
 
     if activation not in ACT_CODES:
         raise ValueError(f"unsupported activation {activation!r}")
@@ -222,16 +273,13 @@ def gated_feed_forward_fp4(x: torch.Tensor, gate_up: FP4Operand, down: FP4Operan
         raise ValueError(f"gate_up must be [2 I, H] and down [H', I]: got {gate_up.shape} and {down.shape}")
     _check_product(x.shape[1], gate_up, gate_up_bias, None, x.shape[0])
     _check_product(down.k, down, down_bias, residual, x.shape[0])
-    grad = torch.is_grad_enabled() and wants_grad(x, gate_up_bias, down_bias, residual)
-    if not (x.is_cuda and x.dtype == torch.bfloat16) or grad:
-        h = gated_activation(linear_fp4(x, gate_up, gate_up_bias), activation)
-        return linear_fp4(h, down, down_bias, residual)
+    if not (x.is_cuda and x.dtype == torch.bfloat16):
+        return gated_feed_forward_fp4_reference(x, gate_up, down, activation, gate_up_bias, down_bias, residual)
     if residual is not None and residual.dtype != torch.bfloat16:
         raise TypeError("residual must be bfloat16 like x")
-    bias = lambda t: None if t is None else view(t).contiguous()  # noqa: E731
-    return ext().fp4_ffn(x if x.stride(1) == 1 else x.contiguous(), gate_up.data, gate_up.scales, gate_up.row_scale,
-                         FORMATS[gate_up.fmt], down.data, down.scales, down.row_scale, FORMATS[down.fmt],
-                         ACT_CODES[activation], bias(gate_up_bias), bias(down_bias), residual, status(x.device))
+    if torch.is_grad_enabled() and wants_grad(x, gate_up_bias, down_bias, residual):
+        return GatedFeedForwardFP4Fn.apply(x, gate_up, down, activation, gate_up_bias, down_bias, residual)
+    return _feed_forward(x, gate_up, down, activation, gate_up_bias, down_bias, residual)
 
 
 # ------------------------------------------------------------ PyTorch statement
@@ -282,12 +330,31 @@ def fake_quantize_reference(x: torch.Tensor, fmt: str) -> torch.Tensor:
     return v.reshape(x.shape[0], -1)[:, :x.shape[1]]
 
 
-def linear_fp4_reference(x, weight: FP4Operand, bias=None, residual=None):
+def _product_reference(x, weight: FP4Operand, bias, residual):
+    """Q(x) Q(W)^T (+ bias) (+ residual) in fp32 for fp32 ``x``."""
+
     y = fake_quantize_reference(x, weight.fmt)
-    y = x.float() + (y - x.float()).detach()  # the quantiser counts as the identity in the backward pass
+    y = x + (y - x).detach()  # the quantiser counts as the identity in the backward pass (the sum is exact)
     y = y @ _unpack_reference(weight).to(y.device).T
     y = y if bias is None else y + bias.float()
-    return (y if residual is None else y + residual.float()).to(x.dtype)
+    return y if residual is None else y + residual.float()
+
+
+def linear_fp4_reference(x, weight: FP4Operand, bias=None, residual=None):
+    return _product_reference(x.float(), weight, bias, residual).to(x.dtype)
+
+
+def gated_feed_forward_fp4_reference(x, gate_up: FP4Operand, down: FP4Operand, activation, gate_up_bias=None, down_bias=None,
+                                     residual=None):
+    """The block in fp32, rounded where the kernels round: h to the type of ``x`` unless both formats are MXFP4, y once."""
+
+    from .nn import _act_reference
+
+    z = _product_reference(x.float(), gate_up, gate_up_bias, None)
+    h = _act_reference(z[:, :down.k], activation) * z[:, down.k:]
+    if gate_up.fmt != "mxfp4" or down.fmt != "mxfp4":
+        h = h.to(x.dtype).float()
+    return _product_reference(h, down, down_bias, residual).to(x.dtype)
 
 
 def _pack_reference(x: torch.Tensor, fmt: str, parts: int) -> FP4Operand:
@@ -338,6 +405,6 @@ def _unpack_reference(op: FP4Operand) -> torch.Tensor:
     return v if op.row_scale is None else v * op.row_scale[:, None]
 
 
-__all__ = ["BLOCK", "FORMATS", "FP4Operand", "LinearFP4Fn", "dequantize", "fake_quantize_reference",
-           "gated_feed_forward_fp4", "gemm", "linear_fp4", "linear_fp4_reference", "quantize", "quantize_reference",
-           "scale_values"]
+__all__ = ["BLOCK", "FORMATS", "FP4Operand", "GatedFeedForwardFP4Fn", "LinearFP4Fn", "dequantize",
+           "fake_quantize_reference", "gated_feed_forward_fp4", "gated_feed_forward_fp4_reference", "gemm", "linear_fp4",
+           "linear_fp4_reference", "quantize", "quantize_reference", "scale_values"]

@@ -117,6 +117,26 @@ def test_feed_forward_statement():
         gated_feed_forward(x, w1, w2, activation="tanh")
 
 
+@pytest.mark.parametrize("fmts", [("mxfp4", "mxfp4"), ("nvfp4", "nvfp4"), ("mxfp4", "nvfp4")])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_feed_forward_rounds_where_the_kernels_round(fmts, dtype):
+    """h is quantised from fp32 in MXFP4 and from the rows' type where NVFP4 is involved; y is rounded once. With and
+    without gradients."""
+
+    g = torch.Generator().manual_seed(8)
+    n = lambda *s: torch.randn(*s, generator=g).to(dtype)  # noqa: E731
+    x, b1, b2, res = n(30, 64), n(96), n(64), n(30, 64)
+    q1, q2 = F.quantize(n(96, 64) / 8, fmts[0], parts=2), F.quantize(n(64, 48) / 7, fmts[1])
+    z = F.fake_quantize_reference(x, fmts[0]) @ F.dequantize(q1, torch.float32).T + b1.float()
+    h = N._act_reference(z[:, :48], "silu") * z[:, 48:]
+    h = h if fmts == ("mxfp4", "mxfp4") else h.to(dtype).float()
+    want = (F.fake_quantize_reference(h, fmts[1]) @ F.dequantize(q2, torch.float32).T + b2.float() + res.float()).to(dtype)
+    run = lambda x: F.gated_feed_forward_fp4(x, q1, q2, activation="silu", gate_up_bias=b1, down_bias=b2, residual=res)  # noqa: E731
+    assert torch.equal(run(x), want)
+    y = run(x.clone().requires_grad_())
+    assert y.requires_grad and torch.equal(y.detach(), want)
+
+
 def test_gated_mlp_keeps_the_separate_layers():
     """Models run the separate layers unless they are asked otherwise: the same bits as before."""
 

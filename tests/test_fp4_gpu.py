@@ -230,6 +230,51 @@ def test_feed_forward_under_grad(fmt):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("t,h,i", [(1, 64, 40), (20, 96, 200), (70, 256, 130), (300, 256, 384)])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_feed_forward_value_and_gradients(fmt, t, h, i, act):
+    """The value is the same with and without gradients. Gradients against those of the separate layers in 64 bits (dh, dz
+    and dx, or the bias gradient, are each rounded to bf16, at most 2^-9 each)."""
+
+    from representax_b200.ops.fp4 import dequantize, gated_feed_forward_fp4, linear_fp4, quantize
+
+    q1, q2 = quantize(_randn(2 * i, h, seed=2, std=h ** -0.5), fmt, parts=2), quantize(_randn(h, i, seed=3, std=i ** -0.5), fmt)
+    x, dy = _randn(t, h, seed=1), _randn(t, h, seed=7)
+    b1, b2, res = _randn(2 * i, seed=4, std=0.2), _randn(h, seed=5), _randn(t, h, seed=6)
+    run = lambda x, b1, b2, res: gated_feed_forward_fp4(x, q1, q2, activation=act, gate_up_bias=b1, down_bias=b2, residual=res)  # noqa: E731
+    want = run(x, b1, b2, res)
+    leaves = [v.clone().requires_grad_() for v in (x, b1, b2, res)]
+    y = run(*leaves)
+    assert torch.equal(y.detach(), want)
+    dx, db1, db2, dres = torch.autograd.grad(y, leaves, dy)
+    _status_ok()
+    z = linear_fp4(x, q1, b1).double().requires_grad_()
+    (dz,) = torch.autograd.grad(_act(z[:, :i], act) * z[:, i:], [z], dy.double() @ dequantize(q2, torch.float32).double())
+    assert _rel(dx, dz @ dequantize(q1, torch.float32).double()) < 3 * 2.0 ** -9
+    assert _rel(db1, dz.sum(0)) < 3 * 2.0 ** -9 and _rel(db2, dy.double().sum(0)) < TOL and torch.equal(dres, dy)
+    for k, leaf in enumerate(leaves):  # one gradient at a time
+        args = [v if j != k else leaf for j, v in enumerate((x, b1, b2, res))]
+        (g,) = torch.autograd.grad(run(*args), [leaf], dy)
+        assert _rel(g, (dx, db1, db2, dres)[k].double()) < 2.0 ** -8
+    wide = torch.nn.Parameter(b1.float())  # an fp32 parameter with an accumulator
+    wide.main_grad = torch.ones_like(wide.data)
+    run(x, wide, b2, res).backward(dy)
+    assert wide.grad is None and _rel(wide.main_grad - 1, dz.sum(0)) < 3 * 2.0 ** -9
+    none = run(x[:0].clone().requires_grad_(), b1, b2, res[:0])
+    assert none.shape == (0, h)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_feed_forward_gradient_of_no_rows(fmt):
+    from representax_b200.ops.fp4 import gated_feed_forward_fp4, quantize
+
+    q1, q2 = quantize(_randn(96, 64, seed=2), fmt, parts=2), quantize(_randn(64, 48, seed=3), fmt)
+    x, b = _randn(0, 64).requires_grad_(), _randn(96, seed=4).requires_grad_()
+    dx, db = torch.autograd.grad(gated_feed_forward_fp4(x, q1, q2, activation="silu", gate_up_bias=b), [x, b], _randn(0, 64))
+    assert dx.shape == (0, 64) and bool((db == 0).all())
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("m", [5, 300])
 def test_nonfinite_rows_stay_rows(fmt, m):
     from representax_b200.ops.fp4 import gated_feed_forward_fp4, linear_fp4, quantize
