@@ -290,9 +290,10 @@ void run_linear(const Operand& a, const Operand& b, const OptTensor& bias, const
   }
 }
 
+// (a clone: a single column counts as contiguous whatever its inner stride says)
 OptTensor unit_rows(const OptTensor& t) {
   if (!t.has_value() || t->dim() != 2 || t->stride(1) == 1) return t;
-  return OptTensor(t->contiguous());
+  return OptTensor(t->clone(at::MemoryFormat::Contiguous));
 }
 
 }  // namespace

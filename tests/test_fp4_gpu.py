@@ -165,6 +165,22 @@ def test_linear_of_parts_and_views(fmt, m):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m", [1, 5, 300])
+def test_single_column_of_any_stride(fmt, m):
+    """One output column, one contraction value: their strides mean nothing, whatever they are."""
+
+    from representax_b200.ops.fp4 import gemm, linear_fp4, quantize
+
+    x, w = _randn(m, 64, seed=1), quantize(_randn(1, 64, seed=2), fmt)
+    res = _randn(7, m, seed=3)[2:3].T  # strides (1, m)
+    want = linear_fp4(x, w, None, res.clone(memory_format=torch.contiguous_format))
+    assert torch.equal(linear_fp4(x, w, None, res), want)
+    assert torch.equal(gemm(quantize(x, fmt), w, residual=res), want)
+    column, thin = _randn(3, m, seed=4)[1:2].T, quantize(_randn(40, 1, seed=5), fmt)
+    assert torch.equal(linear_fp4(column, thin), linear_fp4(column.clone(memory_format=torch.contiguous_format), thin))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("m,n,k", [(1, 40, 64), (70, 203, 301), (300, 512, 256)])
 def test_linear_gradients(fmt, m, n, k):
     """dx = dy Q(W), the bias and residual gradients; one bf16 rounding each."""
