@@ -8,8 +8,9 @@ namespace gemm {
 // GELU (erf form) and its derivative from one exponential: the normal CDF
 // Phi(x) = (1 + erf(x / sqrt 2)) / 2 uses the rational approximation of
 // Abramowitz & Stegun, Handbook of Mathematical Functions, eq. 7.1.26
-// (|error of erf| <= 1.5e-7, far below bf16's resolution), whose exp(-u^2)
-// factor at u = |x| / sqrt 2 is exp(-x^2 / 2), the same exponential the normal
+// (|error of erf| <= 1.5e-7: an absolute bound, far below bf16's resolution of
+// values near one; for x < -4, where Phi is as small as that, the relative error
+// is large), whose exp(-u^2) factor at u = |x| / sqrt 2 is exp(-x^2 / 2), the same exponential the normal
 // density phi(x) needs. gelu = x Phi(x); gelu' = Phi(x) + x phi(x).
 __device__ __forceinline__ void gelu_and_grad(float x, float& gelu, float& grad) {
   const float u = fabsf(x) * 0.70710678118654752440f;
@@ -26,12 +27,6 @@ __device__ __forceinline__ void gelu_and_grad(float x, float& gelu, float& grad)
   const float cdf = 0.5f + 0.5f * copysignf(erf_u, x);
   gelu = x * cdf;
   grad = fmaf(x * 0.39894228040143267794f, e, cdf);
-}
-
-__device__ __forceinline__ float gelu_erf(float x) {
-  float g, d;
-  gelu_and_grad(x, g, d);
-  return g;
 }
 
 }  // namespace gemm

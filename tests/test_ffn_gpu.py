@@ -97,6 +97,55 @@ def test_activations(act, t):
     assert _rel(y, _want(o, act)) < TOL
 
 
+def _between(got, want, error):
+    """Rounding keeps the order, so got lies between the roundings of want - error and want + error."""
+
+    low, high = (want - error).to(torch.bfloat16), (want + error).to(torch.bfloat16)
+    assert got.dtype == torch.bfloat16 and bool(((got >= low) & (got <= high)).all())
+
+
+def _act_grad(g, name):
+    g = g.clone().requires_grad_()
+    if name == "gelu":  # Phi by its complement: exact in the lower tail
+        value = g * 0.5 * torch.special.erfc(-g * 0.5 ** 0.5)
+    elif name == "gelu_tanh":
+        value = g * torch.sigmoid(2 * (2 / torch.pi) ** 0.5 * (g + 0.044715 * g ** 3))
+    else:
+        value = g * torch.sigmoid((1.702 if name == "quick_gelu" else 1.0) * g)
+    (grad,) = torch.autograd.grad(value.sum(), g)
+    return value.detach(), grad
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("t", [1, 40, 300])
+def test_activation_value_by_value(act, t):
+    """act(g) and act'(g) of 512 gates from -8 to 8, each between the bf16 roundings of the ends of its interval. The
+    block is built so that y is h itself (u one, the down projection the identity) and the gate bias's gradient of one
+    row is dz. Before that rounding the activation is off by 2e-5 of itself, the kept factors by 2^-11 more (11
+    bits), and act' next to its zero by the absolute error of its parts, below 2e-6 there."""
+
+    from representax_b200.ops.ffn import gated_feed_forward
+
+    n = 512
+    gates = torch.linspace(-8, 8, n, device=_dev()).to(torch.bfloat16)
+    x = torch.zeros(t, n, dtype=torch.bfloat16, device=_dev())
+    x[:, 0] = 1
+    w1 = torch.zeros(2 * n, n, dtype=torch.bfloat16, device=_dev())
+    w1[:n, 0], w1[n:, 0] = gates, 1
+    w2 = torch.eye(n, dtype=torch.bfloat16, device=_dev())
+    value, grad = _act_grad(gates.double(), act)
+    _between(gated_feed_forward(x, w1, w2, activation=act), value, 2e-5 * value.abs())
+    b1 = torch.zeros(2 * n, dtype=torch.bfloat16, device=_dev(), requires_grad=True)
+    y = gated_feed_forward(x, w1, w2, activation=act, gate_up_bias=b1)
+    _between(y, value, 2e-5 * value.abs())
+    dy = torch.zeros_like(y)
+    dy[t - 1] = 1
+    (db,) = torch.autograd.grad(y, b1, dy)
+    _status_ok()
+    _between(db[:n], grad, (2.0 ** -11 + 2e-5) * grad.abs() + 2e-6 * (grad.abs() < 0.05))
+    _between(db[n:], value, (2.0 ** -11 + 2e-5) * value.abs())
+
+
 @pytest.mark.parametrize("t,h,i", [(1, 64, 64), (7, 96, 200), (33, 128, 72), (64, 512, 384), (257, 264, 1000), (513, 768, 1152)])
 @pytest.mark.parametrize("act", ACTS)
 def test_gradients(t, h, i, act):
