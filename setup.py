@@ -36,6 +36,11 @@ NVCC_FLAGS = [
     "-Xptxas=-v",
 ]
 
+# The shared C++ runtime that torch uses: a compiler whose own directory lacks it would link a second, static copy,
+# and an argument check that formats a number would crash in that copy's locale. Named before the runtime that the
+# compiler adds by itself, it leaves nothing for a static one to resolve; any linker takes it (-nostdlib++ is g++ 13's).
+LINK_FLAGS = ["-l:libstdc++.so.6"]
+
 setup(
     name="representax_b200",
     version="0.1.0",
@@ -44,9 +49,7 @@ setup(
         CUDAExtension(
             name="representax_b200._C",
             sources=[os.path.join(CSRC, s) for s in SOURCES],
-            # The shared C++ runtime that torch uses: a compiler whose own directory lacks it would link a second,
-            # static copy, and an argument check that formats a number would crash in that copy's locale.
-            extra_link_args=["-nostdlib++", "-l:libstdc++.so.6"],
+            extra_link_args=LINK_FLAGS,
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": NVCC_FLAGS},
         )
     ],
