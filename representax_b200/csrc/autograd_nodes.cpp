@@ -3,7 +3,7 @@
 // functions of ops/ffn.py and ops/fp4.py (which serve parameters with fp32
 // accumulators, compute copies or sharding); a small training step spends most
 // of its time on the host, and a node without Python halves that.
-#include <torch/extension.h>
+#include "common.h"
 
 namespace rx {
 
@@ -86,6 +86,7 @@ struct Fp4LinearNode : public torch::autograd::Function<Fp4LinearNode> {
       if (direct) {
         db = at::zeros({dy.size(1)}, dy.options().dtype(at::kFloat));
         colsum_accumulate(dy, db);
+        count_launches((dy.size(1) + 8191) / 8192);  // blocks of columns
       } else {
         db = at::sum(dy, at::IntArrayRef{0}, false, at::kFloat);
       }

@@ -119,6 +119,7 @@ void mx_quantize(const at::Tensor& x, const c10::optional<at::Tensor>& q, const 
 void mx_gemm(const at::Tensor& a, const at::Tensor& sfa, int64_t a_fmt, const at::Tensor& b, const at::Tensor& sfb,
              int64_t b_fmt, int64_t K, at::Tensor& out, int64_t out_mode, const c10::optional<at::Tensor>& bias,
              const c10::optional<at::Tensor>& residual, const at::Tensor& status);
+int64_t kernel_launches();
 void gated_forward(const at::Tensor& x, const at::Tensor& gate_up, const c10::optional<at::Tensor>& bias, at::Tensor& h,
                    const c10::optional<at::Tensor>& saved, const c10::optional<at::Tensor>& exps, int64_t act,
                    const at::Tensor& status);
@@ -234,6 +235,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("int4_gemm", &rx::int4_gemm, "tcgen05 GEMM with the packed INT4 weight expanded in the main loop");
   m.def("mx_quantize", &rx::mx_quantize, "MXFP8 quantiser: row-wise and / or transposed 8-bit data + UE8M0 scales");
   m.def("mx_gemm", &rx::mx_gemm, "tcgen05 block-scaled MXFP8 GEMM (kind::mxf8f6f4.block_scale)");
+  m.def("kernel_launches", &rx::kernel_launches, "kernels launched so far by the feed-forward block and the 4-bit layers");
   m.def("gated_forward", &rx::gated_forward, "tcgen05 gated projection act(x Wg^T) * (x Wu^T), optionally saving for the backward");
   m.def("gated_backward", &rx::gated_backward, "tcgen05 dz = [dh b | dh a], dh = dy Wd, of the gated feed-forward block");
   m.def("few_rows_linear", &rx::few_rows_linear, "bf16 (gated) projection of 1 to 64 token rows");

@@ -9,6 +9,7 @@
 #include <cuda_runtime.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <cstdint>
 
 #define RX_CHECK(cond, ...) TORCH_CHECK(cond, "representax_b200: ", __VA_ARGS__)
@@ -26,6 +27,14 @@ namespace rx {
 // above any legitimate wait in these kernels and short enough that a stuck
 // pipeline unwinds well inside a process-group timeout.
 constexpr uint64_t kWaitBudgetNs = 2000000000ull;
+
+// Kernels launched by the host entries whose number depends on their arguments or whose backward is a node of its
+// own (the feed-forward block and the 4-bit layers); they count where they launch.
+inline std::atomic<int64_t>& launch_count() {
+  static std::atomic<int64_t> count{0};
+  return count;
+}
+inline void count_launches(int64_t n = 1) { launch_count().fetch_add(n, std::memory_order_relaxed); }
 
 inline void check_cuda(const at::Tensor& t, const char* name) {
   RX_CHECK(t.is_cuda(), name, " must be a CUDA tensor");

@@ -82,6 +82,7 @@ gated::Params make_params(int64_t T, int64_t I, int64_t H, int64_t tile_cols, co
 void run(int mode, const gated::Maps& maps, const gated::Params& p, int dev) {
   const cudaError_t e = gated::launch(mode, maps, p, num_sms(dev), dev, at::cuda::getCurrentCUDAStream(dev).stream());
   RX_CHECK(e == cudaSuccess, "gated feed-forward: ", cudaGetErrorString(e));
+  count_launches();
 }
 
 // `t` if the tensor maps can read it (16-byte aligned rows), else a copy.
@@ -103,6 +104,7 @@ at::Tensor weight_gradient(const at::Tensor& dy, const at::Tensor& x, const OptT
   auto product = [&](at::Tensor& out, int64_t mode) {
     gemm_tcgen05(dy, x, out, true, true, 0, mode, 1.0, c10::nullopt, c10::nullopt, c10::nullopt, c10::nullopt, status, 0, 0,
                  0, 0, 0.0, c10::nullopt);
+    count_launches();
   };
   if (acc.has_value()) {
     at::Tensor out = *acc;
@@ -128,11 +130,14 @@ at::Tensor weight_gradient(const at::Tensor& dy, const at::Tensor& x, const OptT
 at::Tensor bias_gradient(const at::Tensor& dy, const OptTensor& acc, at::ScalarType dtype) {
   at::Tensor out = acc.has_value() ? *acc : at::zeros({dy.size(1)}, dy.options().dtype(at::kFloat));
   colsum_accumulate(dy, out);
+  count_launches((dy.size(1) + 8191) / 8192);  // blocks of columns
   if (acc.has_value()) return at::Tensor();
   return dtype == at::kFloat ? out : out.to(dtype);
 }
 
 }  // namespace
+
+int64_t kernel_launches() { return launch_count().load(); }
 
 // bf16 products of few token rows x [T, K] with w [parts * N, K]: parts 1: x w^T (+ bias) (+ residual);
 // parts 2 (gate, up): act(x wg^T + bg) * (x wu^T + bu). `after_producer`: the launch just before, a gated projection,
@@ -180,6 +185,7 @@ void few_rows_linear(const at::Tensor& x, const at::Tensor& w, int64_t parts, in
   const cudaError_t e =
       few::launch(few::kBf16, tx, tw, p, num_sms(dev), dev, at::cuda::getCurrentCUDAStream(dev).stream());
   RX_CHECK(e == cudaSuccess, "few_rows_linear: ", cudaGetErrorString(e));
+  count_launches();
 }
 
 // h [T, I] = act(x Wg^T + bg) * (x Wu^T + bu) for x [T, H] and gate_up = [Wg; Wu] [2 I, H].
@@ -286,11 +292,13 @@ std::vector<at::Tensor> gated_ffn_forward(const at::Tensor& x_in, const at::Tens
   } else {
     gated_forward(x, gate_up, b1, h, c10::nullopt, c10::nullopt, act, status);
   }
-  if (few_down)
+  if (few_down) {
     few_rows_linear(h, down, 1, 0, b2, residual, y, true, status);
-  else
+  } else {
     gemm_tcgen05(h, down, y, false, false, (b2.has_value() ? kBias : 0) | (residual.has_value() ? kResidual : 0), kOutBf16,
                  1.0, b2, c10::nullopt, c10::nullopt, residual, status, 0, 0, 0, 0, 0.0, c10::nullopt);
+    count_launches();
+  }
   return {y, h, saved, exps};
 }
 
@@ -337,6 +345,7 @@ std::vector<at::Tensor> gated_ffn_backward(const at::Tensor& dy_in, const OptTen
           direct ? reinterpret_cast<__nv_bfloat16*>(db.data_ptr()) : nullptr,
           at::cuda::getCurrentCUDAStream(dy.get_device()).stream());
       RX_CHECK(e == cudaSuccess, "gated feed-forward: ", cudaGetErrorString(e));
+      count_launches();
       if (!acc[3].has_value()) out[3] = direct || like[3] == at::kFloat ? db : db.to(like[3]);
     }
     if (need[0]) {
@@ -344,6 +353,7 @@ std::vector<at::Tensor> gated_ffn_backward(const at::Tensor& dy_in, const OptTen
       out[0] = device_empty({dy.size(0), gate_up.size(1)}, at::kBFloat16, dy.get_device());
       gemm_tcgen05(dz, gate_up, out[0], false, true, 0, kOutBf16, 1.0, c10::nullopt, c10::nullopt, c10::nullopt,
                    c10::nullopt, status, 0, 0, 0, 0, 0.0, c10::nullopt);
+      count_launches();
     }
   }
   return out;

@@ -142,6 +142,7 @@ void check_matrix(const at::Tensor& t, const char* name, int64_t rows, int64_t c
 
 void check_launch(cudaError_t e, const char* what) {
   RX_CHECK(e == cudaSuccess, what, ": ", cudaGetErrorString(e));
+  count_launches();
 }
 
 void check_input(const at::Tensor& x, int64_t parts) {
@@ -375,6 +376,7 @@ at::Tensor fp4_linear_dgrad(const at::Tensor& dy_in, const at::Tensor& w, const 
   at::Tensor dx = device_empty({M, ld}, at::kBFloat16, dev).narrow(1, 0, K);
   gemm_tcgen05(dy, wide, dx, false, true, 0, 0, 1.0, c10::nullopt, c10::nullopt, c10::nullopt, c10::nullopt, status, 0, 0, 0,
                0, 0.0, c10::nullopt);
+  count_launches();
   return dx;
 }
 

@@ -30,18 +30,47 @@ class KernelTimeoutError(RuntimeError):
 
 
 # Kernels launched per binding call (used to count our own launches).
-KERNELS_PER_CALL = {"attention_backward": 3, "attention_backward_bias": 3, "grad_norm_sq": 1, "gated_ffn_forward": 2,
-                    "gated_ffn_apply": 2, "gated_ffn_backward": 4, "fp4_linear": 2, "fp4_linear_apply": 2,
-                    "fp4_linear_dgrad": 2, "fp4_ffn": 3}
+KERNELS_PER_CALL = {"attention_backward": 3, "attention_backward_bias": 3, "grad_norm_sq": 1,
+                    "register_status_word": 0}
+# Calls whose number depends on their arguments, or whose backward is a C++ node: the extension counts these itself.
+COUNTED_NATIVELY = ("gated_ffn_forward", "gated_ffn_backward", "gated_ffn_apply", "fp4_quantize", "fp4_dequantize",
+                    "fp4_gemm", "fp4_linear", "fp4_linear_apply", "fp4_linear_dgrad", "fp4_ffn", "kernel_launches")
+KERNELS_PER_CALL.update(dict.fromkeys(COUNTED_NATIVELY, 0))
 
 
 class _CountingModule:
-    """Proxy that counts kernel launches made through the extension."""
+    """Proxy that counts kernel launches made through the extension while ``counting`` is set."""
 
     def __init__(self, module) -> None:
         self._module = module
-        self.launches = 0
-        self.counting = False
+        self._calls = 0     # kernels of counted calls
+        self._native = 0    # the extension's own count, up to where it was last read
+        self._counting = False
+
+    def _collect(self) -> None:
+        now = self._module.kernel_launches()
+        if self._counting:
+            self._calls += now - self._native
+        self._native = now
+
+    @property
+    def counting(self) -> bool:
+        return self._counting
+
+    @counting.setter
+    def counting(self, on: bool) -> None:
+        self._collect()
+        self._counting = on
+
+    @property
+    def launches(self) -> int:
+        self._collect()
+        return self._calls
+
+    @launches.setter
+    def launches(self, count: int) -> None:
+        self._collect()
+        self._calls = count
 
     def __getattr__(self, name):
         fn = getattr(self._module, name)
@@ -50,8 +79,8 @@ class _CountingModule:
         weight = KERNELS_PER_CALL.get(name, 1)
 
         def wrapped(*args, **kwargs):
-            if self.counting:
-                self.launches += weight
+            if self._counting:
+                self._calls += weight
             return fn(*args, **kwargs)
 
         self.__dict__[name] = wrapped  # found without __getattr__ from now on
