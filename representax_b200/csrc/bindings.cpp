@@ -120,14 +120,6 @@ void mx_gemm(const at::Tensor& a, const at::Tensor& sfa, int64_t a_fmt, const at
              int64_t b_fmt, int64_t K, at::Tensor& out, int64_t out_mode, const c10::optional<at::Tensor>& bias,
              const c10::optional<at::Tensor>& residual, const at::Tensor& status);
 int64_t kernel_launches();
-void gated_forward(const at::Tensor& x, const at::Tensor& gate_up, const c10::optional<at::Tensor>& bias, at::Tensor& h,
-                   const c10::optional<at::Tensor>& saved, const c10::optional<at::Tensor>& exps, int64_t act,
-                   const at::Tensor& status);
-void gated_backward(const at::Tensor& dy, const at::Tensor& down, const at::Tensor& saved, const at::Tensor& exps,
-                    at::Tensor& dz, const c10::optional<at::Tensor>& partial, const at::Tensor& status);
-void few_rows_linear(const at::Tensor& x, const at::Tensor& w, int64_t parts, int64_t act,
-                     const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& residual, at::Tensor& out,
-                     bool after_producer, const at::Tensor& status);
 std::vector<at::Tensor> gated_ffn_forward(const at::Tensor& x, const at::Tensor& gate_up, const at::Tensor& down,
                                           const c10::optional<at::Tensor>& gate_up_bias,
                                           const c10::optional<at::Tensor>& down_bias,
@@ -236,9 +228,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mx_quantize", &rx::mx_quantize, "MXFP8 quantiser: row-wise and / or transposed 8-bit data + UE8M0 scales");
   m.def("mx_gemm", &rx::mx_gemm, "tcgen05 block-scaled MXFP8 GEMM (kind::mxf8f6f4.block_scale)");
   m.def("kernel_launches", &rx::kernel_launches, "kernels launched so far by the feed-forward block and the 4-bit layers");
-  m.def("gated_forward", &rx::gated_forward, "tcgen05 gated projection act(x Wg^T) * (x Wu^T), optionally saving for the backward");
-  m.def("gated_backward", &rx::gated_backward, "tcgen05 dz = [dh b | dh a], dh = dy Wd, of the gated feed-forward block");
-  m.def("few_rows_linear", &rx::few_rows_linear, "bf16 (gated) projection of 1 to 64 token rows");
   m.def("fp4_quantize", &rx::fp4_quantize, "MXFP4 / NVFP4 quantiser");
   m.def("fp4_dequantize", &rx::fp4_dequantize, "values of MXFP4 / NVFP4 codes and scales");
   m.def("gated_ffn_forward", &rx::gated_ffn_forward, "forward of the gated feed-forward block");

@@ -135,10 +135,6 @@ at::Tensor bias_gradient(const at::Tensor& dy, const OptTensor& acc, at::ScalarT
   return dtype == at::kFloat ? out : out.to(dtype);
 }
 
-}  // namespace
-
-int64_t kernel_launches() { return launch_count().load(); }
-
 // bf16 products of few token rows x [T, K] with w [parts * N, K]: parts 1: x w^T (+ bias) (+ residual);
 // parts 2 (gate, up): act(x wg^T + bg) * (x wu^T + bu). `after_producer`: the launch just before, a gated projection,
 // wrote x and nothing else that this one reads.
@@ -263,6 +259,10 @@ void gated_backward(const at::Tensor& dy, const at::Tensor& down, const at::Tens
   p.ld_out = dz.stride(0);
   run(gated::kBackward, maps, p, dev);
 }
+
+}  // namespace
+
+int64_t kernel_launches() { return launch_count().load(); }
 
 // The block's forward: {y, h, saved, exps}; h, saved and exps are what the backward needs (saved and
 // exps undefined without `save`).

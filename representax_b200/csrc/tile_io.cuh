@@ -48,33 +48,10 @@ __device__ __forceinline__ void stage_row32_sw64(uint8_t* buf, int lane, const f
   }
 }
 
-// Coalesced load of a 32 x 32 bf16 tile (rows row0.., columns n_base..) into
-// `buf` with the 64-byte swizzle: 16-byte pieces, 4 lanes per 64-byte row
-// segment; rows >= rows_valid and columns >= cols_valid read as zero.
-__device__ __forceinline__ void warp_load_tile32_sw64(uint8_t* buf, const __nv_bfloat16* src, int64_t ld, int row0,
-                                                      int n_base, int rows_valid, int cols_valid, int lane) {
-#pragma unroll
-  for (int it = 0; it < 4; ++it) {
-    const int c = lane + 32 * it;
-    const int row = c >> 2, piece = c & 3;
-    const int m = row0 + row, n = n_base + piece * 8;
-    uint4 w = make_uint4(0u, 0u, 0u, 0u);
-    if (m < rows_valid) {
-      const __nv_bfloat16* g = src + static_cast<int64_t>(m) * ld + n;
-      if (n + 8 <= cols_valid) {
-        w = *reinterpret_cast<const uint4*>(g);
-      } else {
-        __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(&w);
-        for (int k = 0; k < 8; ++k) e[k] = n + k < cols_valid ? g[k] : __float2bfloat16_rn(0.f);
-      }
-    }
-    *reinterpret_cast<uint4*>(buf + row * 64 + ((piece ^ ((row >> 1) & 3)) * 16)) = w;
-  }
-}
-
-// The same 32 x 32 tile in two steps, so the loads of the next tile can be
-// in flight while the current one is computed: fetch into registers (lane
-// holds pieces lane, lane + 32, lane + 64, lane + 96) ...
+// A 32 x 32 bf16 tile (rows row0.., columns n_base..) from global to shared memory, 16-byte pieces, four lanes to a
+// 64-byte row segment; rows >= rows_valid and columns >= cols_valid read as zero. In two steps, so the loads of the next
+// tile can be in flight while the current one is computed: fetch into registers (lane holds pieces lane, lane + 32,
+// lane + 64, lane + 96) ...
 __device__ __forceinline__ void warp_fetch_tile32(const __nv_bfloat16* src, int64_t ld, int row0, int n_base,
                                                   int rows_valid, int cols_valid, int lane, uint4 (&w)[4]) {
 #pragma unroll
