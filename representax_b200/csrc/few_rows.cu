@@ -389,11 +389,14 @@ cudaError_t launch_parts(const CUtensorMap& mx, const CUtensorMap& mw, const Par
   switch (tile_rows(p.T)) {
     case 16: return launch_shape<KIND, PARTS, 16>(mx, mw, p, sms, device, stream);
     case 32: return launch_shape<KIND, PARTS, 32>(mx, mw, p, sms, device, stream);
-    case 64: return launch_shape<KIND, PARTS, 64>(mx, mw, p, sms, device, stream);
+    case 64:
+      if constexpr (PARTS == 1 || KIND == kBf16) return launch_shape<KIND, PARTS, 64>(mx, mw, p, sms, device, stream);
+      break;
     default:
       if constexpr (PARTS == 1) return launch_shape<KIND, PARTS, 128>(mx, mw, p, sms, device, stream);
-      return cudaErrorInvalidValue;  // the hosts send gated products of more rows to the GEMM
+      break;
   }
+  return cudaErrorInvalidValue;  // the hosts send gated products of more rows to the GEMM (`takes`)
 }
 
 template <int KIND>

@@ -282,7 +282,8 @@ std::vector<at::Tensor> gated_ffn_forward(const at::Tensor& x_in, const at::Tens
   const OptTensor residual = residual_in.has_value() ? OptTensor(rows16(*residual_in)) : residual_in;
   const int64_t T = x.size(0), I = down.size(1), H = down.size(0);
   at::Tensor h = device_empty({T, I}, at::kBFloat16, dev), y = device_empty({T, H}, at::kBFloat16, dev), saved, exps;
-  const bool few_gated = !save && few::takes(T, I, (H + 63) / 64, true), few_down = few::takes(T, H, (I + 63) / 64, false);
+  const bool few_gated = !save && few::takes(few::kBf16, T, I, (H + 63) / 64, true);
+  const bool few_down = few::takes(few::kBf16, T, H, (I + 63) / 64, false);
   if (save) {
     saved = device_empty({saved_tiles(T, I), 2, 32, 32}, at::kHalf, dev);
     exps = device_empty({saved_tiles(T, I), 32}, at::kShort, dev);

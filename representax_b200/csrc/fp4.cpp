@@ -240,7 +240,7 @@ void run_product(const Operand& a, const Operand& b, int64_t act, const OptTenso
     p.timeout_ns = kWaitBudgetNs;
   };
   const CUtensorMap tb = make_tmap_2d_u8(b.q, b.all_rows(), b.code_bytes(), b.ldq, 128);
-  if (few::takes(M, N, (K + 255) / 256, b.parts == 2)) {
+  if (few::takes(a.fmt, M, N, (K + 255) / 256, b.parts == 2)) {
     const CUtensorMap ta = make_tmap_2d_u8(a.q, M, a.code_bytes(), a.ldq, few::tile_rows(M));
     few::Params p{};
     fill(p);

@@ -87,6 +87,17 @@ def test_forward(t, h, i, bias):
     assert _rel(y, _want(o, act)) < TOL
 
 
+@pytest.mark.parametrize("t,h,i", [(32, 64, 2568), (33, 64, 2560), (33, 64, 2568), (64, 72, 2560), (64, 136, 1000), (65, 64, 2560),
+                                   (65, 200, 520), (200, 200, 1600), (600, 200, 1600), (600, 264, 1600), (2000, 256, 1600),
+                                   (300, 776, 2504)])
+def test_forward_on_both_sides_of_the_few_row_bounds(t, h, i):
+    o, _ = _operands(t, h, i)
+    y = _run(o, "silu")
+    _status_ok()
+    assert _rel(y, _want(o, "silu")) < TOL
+    assert max(_rel(y[r:r + 16], _want(o, "silu")[r:r + 16]) for r in range(0, t, 16)) < 2 * TOL
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("t", [3, 70])
 def test_activations(act, t):

@@ -145,6 +145,20 @@ def test_linear(fmt, m, n, k):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m,n,k", [(16, 72, 64), (17, 72, 64), (32, 72, 700), (33, 72, 700), (33, 72, 800), (64, 300, 1100), (65, 300, 1700),
+                                   (65, 300, 2000), (300, 1024, 2000), (300, 1100, 2000), (2000, 200, 2000)])
+def test_linear_on_both_sides_of_the_few_row_bounds(fmt, m, n, k):
+    from representax_b200.ops.fp4 import dequantize, linear_fp4, quantize
+
+    x, w, res = _randn(m, k, seed=m + k), _randn(n, k, seed=n, std=k ** -0.5), _randn(m, n, seed=2)
+    wq = quantize(w, fmt)
+    y = linear_fp4(x, wq, None, res)
+    _status_ok()
+    want = dequantize(quantize(x, fmt), torch.float32).double() @ dequantize(wq, torch.float32).double().T + res.double()
+    assert _rel(y, want) < TOL
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("m", [3, 200])
 def test_linear_of_parts_and_views(fmt, m):
     from representax_b200.ops.fp4 import linear_fp4, quantize
