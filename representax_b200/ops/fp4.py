@@ -273,6 +273,8 @@ def gated_feed_forward_fp4(x: torch.Tensor, gate_up: FP4Operand, down: FP4Operan
         raise ValueError(f"gate_up must be [2 I, H] and down [H', I]: got {gate_up.shape} and {down.shape}")
     _check_product(x.shape[1], gate_up, gate_up_bias, None, x.shape[0])
     _check_product(down.k, down, down_bias, residual, x.shape[0])
+    if not x.device == gate_up.device == down.device:
+        raise ValueError(f"x is on {x.device}, the weights on {gate_up.device} and {down.device}")
     if not (x.is_cuda and x.dtype == torch.bfloat16):
         return gated_feed_forward_fp4_reference(x, gate_up, down, activation, gate_up_bias, down_bias, residual)
     if residual is not None and residual.dtype != torch.bfloat16:

@@ -175,6 +175,21 @@ def test_weights_swapped_in_a_model(fmt):
         FP4Weight(torch.zeros(4, 32), fmt="int4")
 
 
+def test_feed_forward_refuses_weights_of_another_device():
+    import copy
+
+    x, q1, q2 = torch.randn(4, 64), F.quantize(torch.randn(96, 64), parts=2), F.quantize(torch.randn(64, 48))
+    for first, second in ((True, False), (False, True), (True, True)):
+        ops = []
+        for op, away in ((q1, first), (q2, second)):
+            op = copy.copy(op)
+            if away:
+                op.data, op.scales, op.row_scale = (t.to("meta") for t in (op.data, op.scales, op.row_scale))
+            ops.append(op)
+        with pytest.raises(ValueError, match="weights on"):
+            F.gated_feed_forward_fp4(x, *ops, activation="silu")
+
+
 def test_refusals():
     x = torch.randn(4, 64)
     w = F.quantize(torch.randn(32, 64))
