@@ -116,6 +116,8 @@ def dequantize(op: FP4Operand, dtype: torch.dtype = torch.bfloat16, out: torch.T
 
     if out is None:
         out = torch.empty(op.rows, op.k, dtype=dtype, device=op.device)
+    elif out.shape != op.shape:
+        raise ValueError(f"out must be {op.shape}, got {tuple(out.shape)}")
     if not op.data.is_cuda:
         return out.copy_(_unpack_reference(op))
     ext().fp4_dequantize(op.data, op.scales, op.row_scale, op.parts, FORMATS[op.fmt], out)

@@ -190,6 +190,13 @@ def test_feed_forward_refuses_weights_of_another_device():
             F.gated_feed_forward_fp4(x, *ops, activation="silu")
 
 
+def test_dequantize_refuses_an_output_of_another_shape():
+    op = F.quantize(torch.randn(4, 40))
+    for shape in ((4, 50), (4, 39), (5, 40), (160,), (1, 40), (2, 4, 40)):  # (50 columns take as many bytes of codes as 40)
+        with pytest.raises(ValueError, match="out must be"):
+            F.dequantize(op, out=torch.empty(shape))
+
+
 def test_refusals():
     x = torch.randn(4, 64)
     w = F.quantize(torch.randn(32, 64))
