@@ -76,6 +76,8 @@ class FP4Operand:
     def part(self, index: int) -> "FP4Operand":
         """One of the parts as an operand of its own (views, no copy)."""
 
+        if not 0 <= index < self.parts:
+            raise IndexError(f"part {index} of {self.parts}")
         n, t = self.rows // self.parts, self.scales.shape[0] // self.parts
         return FP4Operand(self.data[index * n:(index + 1) * n], self.scales[index * t:(index + 1) * t],
                           None if self.row_scale is None else self.row_scale[index * n:(index + 1) * n], self.fmt, self.k)

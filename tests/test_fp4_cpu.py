@@ -197,6 +197,14 @@ def test_dequantize_refuses_an_output_of_another_shape():
             F.dequantize(op, out=torch.empty(shape))
 
 
+def test_part_refuses_an_index_out_of_range():
+    op = F.quantize(torch.randn(4, 40), parts=2)
+    for index in (-1, 2):
+        with pytest.raises(IndexError, match="of 2"):
+            op.part(index)
+    assert op.part(1).rows == 2
+
+
 def test_refusals():
     x = torch.randn(4, 64)
     w = F.quantize(torch.randn(32, 64))
