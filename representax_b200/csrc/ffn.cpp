@@ -2,9 +2,8 @@
 // and the block's forward and backward as one call each (its launches in a row,
 // intermediates from the caching allocator on the current stream), so that a
 // small call is not bound by the host.
-#include <ATen/cuda/EmptyTensor.h>
-
 #include "common.h"
+#include "device_empty.h"
 #include "few_rows.h"
 #include "gated.h"
 
@@ -20,12 +19,6 @@ void colsum_accumulate(const at::Tensor& x, at::Tensor& out);
 namespace {
 
 using OptTensor = c10::optional<at::Tensor>;
-
-// Uninitialised device memory straight from the CUDA allocator (at::empty without the dispatcher's share of the
-// host time).
-at::Tensor device_empty(at::IntArrayRef sizes, at::ScalarType dtype, int device) {
-  return at::detail::empty_cuda(sizes, dtype, at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device)), c10::nullopt);
-}
 
 // The epilogue and output codes of gemm_kernel.cuh.
 constexpr int64_t kBias = 1, kResidual = 8;

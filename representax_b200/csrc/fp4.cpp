@@ -2,9 +2,8 @@
 // token rows: argument checks, tensor maps, dispatch.
 #include "fp4.h"
 
-#include <ATen/cuda/EmptyTensor.h>
-
 #include "common.h"
+#include "device_empty.h"
 #include "few_rows.h"
 
 namespace rx {
@@ -18,12 +17,6 @@ void gemm_tcgen05(const at::Tensor& A, const at::Tensor& B, at::Tensor& C, bool 
 namespace {
 
 using OptTensor = c10::optional<at::Tensor>;
-
-// Uninitialised device memory straight from the CUDA allocator (at::empty without the dispatcher's share of the
-// host time).
-at::Tensor device_empty(at::IntArrayRef sizes, at::ScalarType dtype, int device) {
-  return at::detail::empty_cuda(sizes, dtype, at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device)), c10::nullopt);
-}
 
 constexpr int kMx = 1, kNv = 2;
 
