@@ -22,10 +22,11 @@
 //
 // Bound by HBM: floor = bytes of W / copy bandwidth, and by the 4 us that a launch, the
 // first bytes, the cluster barriers and the reduction take whatever the size. One
-// token, K 2048, [6144 gate; 6144 up] bf16 (50 MB, floor 7.8 us): 11.4 us; down
-// projection of it (25 MB, floor 3.9 us) 8.9 us; the two in a row 19.5 us; NVFP4
-// 12288 outputs (14 MB) 6.6 us. 128 tokens through the down projection 16.8 us
-// against 35 us of the 256-row GEMM, which has only 8 tiles there. Every wait is bounded.
+// token, weights of several layers in turn: K 2048, [6144 gate; 6144 up] bf16 (50 MB,
+// floor 7.8 us) 11.9 us; down projection of it (25 MB, floor 3.9 us) 9.0 us; the two in a
+// row 19.4 us (14.6 when one layer's weights stay in L2); NVFP4 12288 outputs (14 MB) with
+// the quantiser 8.8 us. 128 tokens through the down projection 15.4 us against 36.5 us of
+// the 256-row GEMM, which has only 8 tiles there. Every wait is bounded.
 #include "few_rows.h"
 
 #include <algorithm>

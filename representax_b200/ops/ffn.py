@@ -4,8 +4,9 @@
 token rows, with the gate and up projections in one weight ``[Wg; Wu]``.
 
 bf16 CUDA rows run hand-written kernels: one launch computes both
-projections, the activation and the product (``csrc/gated.cu``; up to 32 rows
-the weight-streaming kernel of ``csrc/few_rows.cu``), a second one the down projection with bias and residual. The gate and up projections
+projections, the activation and the product (``csrc/gated.cu``; up to 32 rows, or
+64 of narrow blocks, the weight-streaming kernel of ``csrc/few_rows.cu``), a second
+one the down projection with bias and residual. The gate and up projections
 are never written. For the backward pass the first launch also keeps
 ``act(g)`` and ``u act'(g)`` in 16 bits; the gradient of the block then takes
 one launch for ``dz = [dh u act'(g) | dh act(g)]`` with ``dh = dy Wd`` (``dh`` is
